@@ -20,7 +20,8 @@ BENCH_LIB = os.path.join(HERE, "libbreccia_kv_bench.so")
 # the calls of a serving loop for Python callers, past ctypes (csrc/hot_calls.cpp)
 HOT_MODULE = os.path.join(HERE, "_hot" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
-SOURCES = ["allocator.cpp", "prefix_tree.cpp", "api.hip", "kv_move.hip", "decode_attn.hip", "decode_attn_mfma.hip", "prefill_attn.hip", "select.hip"]
+SOURCES = ["allocator.cpp", "prefix_tree.cpp", "api.hip", "kv_move.hip", "decode_attn.hip", "decode_attn_mfma.hip", "prefill_attn.hip", "select.hip", "f8p_move.hip",
+           "f8p_decode.hip", "f8p_chunk.hip"]
 ARCH = "gfx950"
 # Packed-FP32 VALU forms are switched off for every kernel in this library.
 HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
@@ -28,7 +29,7 @@ HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-
 # The chunk attention kernel fills both halves of a wave's register file.  By default every matrix product of
 # such a kernel accumulates in the upper half, which the VALU cannot read; this option lets the register allocator
 # decide, product by product.
-FILE_FLAGS = {"prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {"prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "f8p_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _hipcc() -> str:

@@ -19,6 +19,7 @@
 #include <unistd.h>
 
 #include "bkv_internal.hpp"
+#include "f8p.hpp"
 
 namespace bkv {
 
@@ -393,11 +394,13 @@ bkv_status bkv_pool_create(const bkv_pool_desc* d, bkv_pool** out) {
     if (d->page_cells != 16)
         return fail(BKV_ERR_INVALID, sfmt("pool_create: page_cells %lld; pages are 16 cells",
                                           d->page_cells));
-    if (d->layout < BKV_LAYOUT_F16 || d->layout > BKV_LAYOUT_I8H)
+    if (d->layout < BKV_LAYOUT_F16 || d->layout > BKV_LAYOUT_F8P)
         return fail(BKV_ERR_INVALID, sfmt("pool_create: unknown layout %lld", d->layout));
     if (d->layout == BKV_LAYOUT_I8H && d->head_dim != 256)
         return fail(BKV_ERR_INVALID, "pool_create: the int8 + f16-scale layout is built for "
                                      "head_dim 256 (272-byte rows keep 16-byte alignment)");
+    if (d->layout == BKV_LAYOUT_F8P && d->head_dim != kF8Hd)
+        return fail(BKV_ERR_INVALID, sfmt("pool_create: the e4m3 layout is built for head_dim 256, not %lld", d->head_dim));
     if ((int64_t)d->n_pages * d->page_cells >= (int64_t)1 << 31)
         return fail(BKV_ERR_INVALID, "pool_create: n_pages * page_cells must stay below 2^31");
 
@@ -418,6 +421,10 @@ bkv_status bkv_pool_create(const bkv_pool_desc* d, bkv_pool** out) {
     const uint64_t rows_per_page = (uint64_t)d->n_kv_head * (uint64_t)d->page_cells;
     g.k_page_bytes = rows_per_page * g.k_row_bytes;
     g.v_page_bytes = rows_per_page * g.v_row_bytes;
+    if (d->layout == BKV_LAYOUT_F8P) {
+        g.k_page_bytes = f8p_k_page_bytes(d->n_kv_head);
+        g.v_page_bytes = f8p_v_page_bytes(d->n_kv_head);
+    }
     g.k_pool_bytes = g.k_page_bytes * (uint64_t)d->n_pages;
     g.v_pool_bytes = g.v_page_bytes * (uint64_t)d->n_pages;
     try {
@@ -855,6 +862,13 @@ static bkv_status build_append_batch(bkv_pool* p, int32_t layer, int32_t n_seqs,
         b.src0[i] = (int32_t)total;
         total += n_tokens[i];
         max_tok = std::max(max_tok, n_tokens[i]);
+        // A page of the e4m3 layout is written as a whole: two entries of a call must not meet in one.
+        if (p->g.layout == BKV_LAYOUT_F8P && n_tokens[i] > 0)
+            for (int j = 0; j < i; ++j)
+                if (seqs[j] == seqs[i] && n_tokens[j] > 0 && pos0[i] / p->g.page_cells <= (pos0[j] + n_tokens[j] - 1) / p->g.page_cells &&
+                    pos0[j] / p->g.page_cells <= (end - 1) / p->g.page_cells)
+                    return fail(BKV_ERR_INVALID, sfmt("append: entries %lld and %lld of the call write the same page of sequence %lld, "
+                                                      "which this layout writes as a whole; one entry, or two calls", j, i, seqs[i]));
     }
     b.n = n_seqs;
     if (total > ((int64_t)1 << 30))
@@ -1053,7 +1067,13 @@ static bkv_status decode_attn_common(bkv_pool* p, int32_t layer, int32_t n, cons
         a.id_stride = id_stride;
         a.max_ids = max_ids;
     }
-    if (step) {
+    if (step && p->g.layout == BKV_LAYOUT_F8P) {
+        // a new row changes its page's scale, and with it the page: a launch ahead of the attention
+        AppendBatch rows{};
+        rows.n = n;
+        for (int i = 0; i < n; ++i) rows.row[i] = b.row[i], rows.pos0[i] = b.pos[i], rows.n_tok[i] = 1, rows.src0[i] = i;
+        BKV_HIP(launch_append_f8p(p, layer, rows, new_k_dev, new_v_dev, false, S(stream)));
+    } else if (step) {
         a.new_k = new_k_dev;
         a.new_v = new_v_dev;
     }
@@ -1295,8 +1315,12 @@ bkv_status bkv_step_plan_decode(bkv_step_plan* pl, int32_t layer, const float* k
     a.gate_head_stride = gate_head_stride;
     a.scale = scale;
     a.out = out_dev;
-    a.new_k = k_new_dev;
-    a.new_v = v_new_dev;
+    if (p->g.layout == BKV_LAYOUT_F8P) {
+        BKV_HIP(launch_append_f8p_desc(p, layer, &pl->dev->b, pl->n, k_new_dev, v_new_dev, S(stream)));
+    } else {
+        a.new_k = k_new_dev;
+        a.new_v = v_new_dev;
+    }
     a.ws_o = pl->part_o;
     a.ws_ml = pl->part_ml;
     a.timed = false;
@@ -1386,7 +1410,8 @@ bkv_status bkv_prefill_attn(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
             return fail(BKV_ERR_INVALID, "prefill_attn: more than 2^24 tokens in one call");
     }
     b.n = n_seqs;
-    const bool f16 = p->g.layout == BKV_LAYOUT_F16;
+    // e4m3 pages take blocks and cuts like f16 ones: one or two tiles of rows a wave
+    const bool f16 = p->g.layout == BKV_LAYOUT_F16 || p->g.layout == BKV_LAYOUT_F8P;
     const int64_t rows_per_wg = prefill_rows_per_wg(f16, wgs, p->n_cu);
     order_chunks(b, p->g.n_kv, (int32_t)group, (int32_t)rows_per_wg);
     bkv_status st = need_device(p);
@@ -2038,8 +2063,68 @@ bkv_status bkv_gather(bkv_pool* p, int32_t layer, int32_t seq, int64_t cell0, in
     if (!k_out_dev || !v_out_dev) return fail(BKV_ERR_INVALID, "gather: NULL output");
     st = flush_tables(p, S(stream));
     if (st != BKV_OK) return st;
+    if (p->g.layout == BKV_LAYOUT_F8P) {
+        AppendBatch b{};
+        b.n = 1;
+        b.row[0] = seq, b.pos0[0] = (int32_t)cell0, b.n_tok[0] = (int32_t)n;
+        BKV_HIP(launch_read_rows(p, layer, b, (int32_t)n, k_out_dev, v_out_dev, false, S(stream)));
+        return BKV_OK;
+    }
     BKV_HIP(launch_gather(p, layer, seq, cell0, n, k_out_dev, v_out_dev, S(stream)));
     return BKV_OK;
+}
+
+static bkv_status read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const int32_t* seqs, const int64_t* cell0, const int32_t* n_cells,
+                            void* k_out_dev, void* v_out_dev, bool to_f16, void* stream) {
+    if (!p) return fail(BKV_ERR_INVALID, "read_rows: NULL pool");
+    if (layer < 0 || layer >= p->g.n_layers)
+        return fail(BKV_ERR_RANGE, sfmt("read_rows: layer %lld is outside 0..%lld", layer, p->g.n_layers));
+    if (n_seqs < 0 || n_seqs > BKV_MAX_BATCH)
+        return fail(BKV_ERR_INVALID, sfmt("read_rows: %lld sequences in one call; the limit is %lld", n_seqs, BKV_MAX_BATCH));
+    if (n_seqs > 0 && (!seqs || !cell0 || !n_cells))
+        return fail(BKV_ERR_INVALID, "read_rows: NULL sequence / cell / count array");
+    AppendBatch b{};
+    b.n = n_seqs;
+    int64_t total = 0;
+    int32_t most = 0;
+    for (int i = 0; i < n_seqs; ++i) {
+        if (!p->alloc->seq_valid(seqs[i])) return fail(BKV_ERR_RANGE, sfmt("read_rows: sequence %lld is not live", seqs[i]));
+        if (n_cells[i] < 0 || cell0[i] < 0 || cell0[i] > p->alloc->seq_capacity(seqs[i]) - n_cells[i])
+            return fail(BKV_ERR_RANGE, sfmt("read_rows: %lld cells from %lld on of sequence %lld, which holds %lld", n_cells[i], cell0[i],
+                                            seqs[i], p->alloc->seq_capacity(seqs[i])));
+        if (n_cells[i] > 0) {
+            const int32_t* row = p->alloc->seq_table(seqs[i]);
+            for (int64_t c = cell0[i] / p->g.page_cells; c <= (cell0[i] + n_cells[i] - 1) / p->g.page_cells; ++c)
+                if (row[c] < 0)
+                    return fail(BKV_ERR_STATE, sfmt("read_rows: logical page %lld of sequence %lld is swapped out", c, seqs[i]));
+        }
+        b.row[i] = seqs[i];
+        b.pos0[i] = (int32_t)cell0[i];
+        b.n_tok[i] = n_cells[i];
+        b.src0[i] = (int32_t)total;
+        total += n_cells[i];
+        most = std::max(most, n_cells[i]);
+        if (total > ((int64_t)1 << 30)) return fail(BKV_ERR_INVALID, "read_rows: more than 2^30 cells in one call");
+    }
+    bkv_status st = need_device(p);
+    if (st != BKV_OK) return st;
+    if (total == 0) return flush_tables(p, S(stream));
+    if (!k_out_dev || !v_out_dev || !aligned16(k_out_dev) || !aligned16(v_out_dev))
+        return fail(BKV_ERR_INVALID, "read_rows: output device pointers must be non-NULL and 16-byte aligned");
+    st = flush_tables(p, S(stream));
+    if (st != BKV_OK) return st;
+    BKV_HIP(launch_read_rows(p, layer, b, most, k_out_dev, v_out_dev, to_f16, S(stream)));
+    return BKV_OK;
+}
+
+bkv_status bkv_read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const int32_t* seqs, const int64_t* cell0, const int32_t* n_cells,
+                         float* k_out_dev, float* v_out_dev, void* stream) {
+    return read_rows(p, layer, n_seqs, seqs, cell0, n_cells, k_out_dev, v_out_dev, false, stream);
+}
+
+bkv_status bkv_read_rows_f16(bkv_pool* p, int32_t layer, int32_t n_seqs, const int32_t* seqs, const int64_t* cell0, const int32_t* n_cells,
+                             uint16_t* k_out_dev, uint16_t* v_out_dev, void* stream) {
+    return read_rows(p, layer, n_seqs, seqs, cell0, n_cells, k_out_dev, v_out_dev, true, stream);
 }
 
 // ---- per-kernel timing ---------------------------------------------------------------

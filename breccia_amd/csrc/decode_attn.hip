@@ -287,7 +287,8 @@ hipError_t launch_decode_attn(bkv_pool* p, int32_t layer, const AttnBatch& b, co
     // the events ride on the dispatch
     hipEvent_t ev_start = nullptr, ev_stop = nullptr;
     if (a.timed) (void)timer_dispatch_events(p, BKV_STAGE_ATTN_SPLIT, &ev_start, &ev_stop);
-    hipError_t err = launch_decode_attn_mfma(kp, b, p->g.layout, step, sel, total, stream, ev_start, ev_stop);
+    hipError_t err = p->g.layout == BKV_LAYOUT_F8P ? launch_decode_attn_f8p(kp, b, sel, total, stream, ev_start, ev_stop)
+                                                   : launch_decode_attn_mfma(kp, b, p->g.layout, step, sel, total, stream, ev_start, ev_stop);
     if (err != hipSuccess) return err;
     MergeParams mp;
     mp.bd = a.desc;

@@ -821,6 +821,7 @@ static hipError_t launch_append_from(bkv_pool* p, int32_t layer, const Batch& b,
 
 hipError_t launch_append(bkv_pool* p, int32_t layer, const AppendBatch& b, int32_t max_tok,
                          const void* k, const void* v, bool src_is_f16, hipStream_t stream) {
+    if (p->g.layout == BKV_LAYOUT_F8P) return launch_append_f8p(p, layer, b, k, v, src_is_f16, stream);
     hipError_t err = hipSuccess;
     with_batch(b, [&](const auto& batch) {
         err = src_is_f16 ? launch_append_from(p, layer, batch, max_tok, (const uint16_t*)k, (const uint16_t*)v, stream)
@@ -833,6 +834,8 @@ hipError_t launch_append_kprep(bkv_pool* p, int32_t layer, const AppendBatch& b,
                                const float* k, const float* v, const float* gamma, float eps,
                                const float* table, int32_t n_rot, int32_t max_pos,
                                const int32_t* positions, hipStream_t stream) {
+    if (p->g.layout == BKV_LAYOUT_F8P)
+        return launch_append_kprep_f8p(p, layer, b, k, v, gamma, eps, table, n_rot, max_pos, positions, stream);
     const MoveGeom g = move_geom(p);
     const KPrepParams kp{gamma, table, positions, eps, n_rot, max_pos,
                          g.n_kv > 1 ? (uint32_t)(((1ull << 32) + (uint64_t)g.n_kv - 1) / (uint64_t)g.n_kv) : 0u};

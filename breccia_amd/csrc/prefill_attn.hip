@@ -67,6 +67,7 @@
 #include "bkv_internal.hpp"
 #include "gate.hpp"
 #include "lane_groups.hpp"
+#include "prefill_common.hpp"
 #include "quant_decode.hpp"
 
 namespace bkv {
@@ -93,30 +94,6 @@ typedef short tr_s4 __attribute__((__vector_size__(8)));  // what the transposin
 typedef __attribute__((address_space(3))) tr_s4* lds_tr_ptr;
 typedef const __attribute__((address_space(1))) uint8_t* page_ptr;  // said to be global memory: its address goes through integers
 
-struct PrefillKernelParams {
-    PrefillBatch b;
-    const uint8_t* kpool;
-    const uint8_t* vpool;
-    const int32_t* tables;
-    const float* q;     // [sum n_tok][n_q][256]
-    const float* gate;  // optional
-    float* out;         // [sum n_tok][n_q][256]
-    int64_t gate_tok_stride, gate_head_stride;
-    int32_t max_pages_per_seq, n_kv, n_q, group;
-    float scale_log2e;
-    uint32_t group_inverse, n_kv_inverse;  // floor((2^32 - 1) / n), for divided_by
-    int32_t gate_in_fours;                 // four gate values can be read at once
-    int32_t by_xcd;  // work-groups are dealt to the chip's 8 dies so that each die sees few (entry, kv head) units
-};
-
-// A cut call: a work-group walks one range of its block's pages and leaves a partial result,
-// prefill_merge_kernel puts the ranges of a row together.
-struct PrefillSplitParams : PrefillKernelParams {
-    PrefillSplit s;
-    float* part_o;   // [slot][row of the block][256], relative to the range's own softmax reference
-    float* part_ml;  // [slot][row of the block][reference, denominator]
-};
-
 // The chip is 8 dies (XCDs), each with an L2 of its own, and work-group i runs on die i % 8.
 // Every work-group of one (entry, kv head) unit walks the same K/V pages, so the dies are given
 // whole units: with 8 or more units, die x serves units x, x + 8, ...; with fewer, unit u is
@@ -132,48 +109,6 @@ __device__ __forceinline__ f4 mfma32(h8 a, h8 b, f4 c) {
 __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
     hi = (_Float16)x;
     lo = (_Float16)(x - (float)hi);
-}
-
-// x / n and the rest, for x >= 0: the inverse is below 2^32 / n by 1 at most, so the product's quotient is right or one
-// too small.  (A division by a number that only the launch knows is some 40 instructions.)
-__device__ __forceinline__ int divided_by(int x, int n, uint32_t inverse, int& rest) {
-    int q = (int)__umulhi((uint32_t)x, inverse);
-    rest = x - q * n;
-    if (rest >= n) ++q, rest -= n;
-    return q;
-}
-__device__ __forceinline__ int divided_by(int x, int n, uint32_t inverse) {
-    int rest;
-    return divided_by(x, n, inverse, rest);
-}
-
-// The arguments' cache lines, asked for at once as a kernel begins: left to where each field is used, they are a chain of
-// trips to memory (41 tokens behind 517 cells through 12 layers: 234 us, 218 with this and `held`).
-template <typename S>
-__device__ __forceinline__ void now(const PrefillBatch& b, int n_kv, const S& at_end) {
-    asm volatile("" : : "s"(b.row[0]), "s"(b.pos0[0]), "s"(b.n_tok[0]), "s"(b.src0[0]), "s"(b.wg_base[0]), "s"(n_kv), "s"(at_end));
-}
-__device__ __forceinline__ void now(const PrefillSplit& s) {
-    asm volatile("" : : "s"(s.pps), "s"(s.splits[0]), "s"(s.wg_base[0]), "s"(s.unit_base[0]), "s"(s.slot_base[0]));
-}
-// keeps an argument in registers from here on instead of asking for it again
-template <typename T>
-__device__ __forceinline__ T held(T x) {
-    asm volatile("" : "+s"(x));
-    return x;
-}
-// A pointer that came through `held` is not known to be to global memory any more: used as it is, each access is a flat one,
-// which LDS counts too and which are waited for together.
-template <typename T>
-__device__ __forceinline__ __attribute__((address_space(1))) T* in_global(T* p) {
-    return (__attribute__((address_space(1))) T*)p;
-}
-
-// what lane i has in x
-__device__ __forceinline__ uint64_t lane_value(uint64_t x, int i) {
-    const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)x, i);
-    const unsigned hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(x >> 32), i);
-    return (uint64_t)hi << 32 | lo;
 }
 
 // two f32 numbers as f16, rounded to nearest
@@ -1205,13 +1140,16 @@ hipError_t launch_split(bkv_pool* p, const PrefillSplitParams& kp, hipStream_t s
                   dim3((unsigned)kp.s.wg_base[kp.b.n]), dim3(256), 0, stream, kp);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    const unsigned rows = (unsigned)kp.s.unit_base[kp.b.n] * kRows;
-    launch_staged(p, BKV_STAGE_ATTN_MERGE, prefill_merge_kernel, dim3(rows / kMergeWaves), dim3(64 * kMergeWaves), 0,
-                  stream, kp, (int32_t)kRows);
-    return hipGetLastError();
+    return launch_prefill_merge(p, kp, (int32_t)kRows, stream);
 }
 
 }  // namespace
+
+hipError_t launch_prefill_merge(bkv_pool* p, const PrefillSplitParams& kp, int32_t rows_per_wg, hipStream_t stream) {
+    const unsigned rows = (unsigned)(kp.s.unit_base[kp.b.n] * rows_per_wg);
+    launch_staged(p, BKV_STAGE_ATTN_MERGE, prefill_merge_kernel, dim3(rows / kMergeWaves), dim3(64 * kMergeWaves), 0, stream, kp, rows_per_wg);
+    return hipGetLastError();
+}
 
 hipError_t launch_prefill_attn(bkv_pool* p, int32_t layer, const PrefillBatch& b, const AttnArgs& a,
                                int32_t rows_per_wg, const PrefillSplit* split, const ChunkWorkspace* ws, hipStream_t stream) {
@@ -1241,6 +1179,7 @@ hipError_t launch_prefill_attn(bkv_pool* p, int32_t layer, const PrefillBatch& b
         sp.s = *split;
         sp.part_o = ws->o;
         sp.part_ml = ws->ml;
+        if (p->g.layout == BKV_LAYOUT_F8P) return launch_chunk_attn_f8p(p, sp, rows_per_wg, true, (uint32_t)split->wg_base[b.n], stream);
         if (p->g.layout == BKV_LAYOUT_Q8V) return launch_split<BKV_LAYOUT_Q8V, 2>(p, sp, stream);
         if (p->g.layout == BKV_LAYOUT_I8H) return launch_split<BKV_LAYOUT_I8H, 2>(p, sp, stream);
         return launch_split<BKV_LAYOUT_F16, 1>(p, sp, stream);
@@ -1253,6 +1192,7 @@ hipError_t launch_prefill_attn(bkv_pool* p, int32_t layer, const PrefillBatch& b
         kp.by_xcd = 1;
         grid = (int32_t)(share * kXcds);
     }
+    if (p->g.layout == BKV_LAYOUT_F8P) return launch_chunk_attn_f8p(p, sp, rows_per_wg, false, (uint32_t)grid, stream);
     if (p->g.layout == BKV_LAYOUT_Q8V)
         launch_staged(p, BKV_STAGE_PREFILL_ATTN, prefill_attn_kernel<BKV_LAYOUT_Q8V, 2>, dim3((unsigned)grid), dim3(256), 0,
                       stream, kp);

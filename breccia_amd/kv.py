@@ -526,6 +526,16 @@ class Pool:
                                               else pairs, dtype=np.int32).reshape(-1, 2))
         check(lib.bkv_page_copy(self.handle, _pointer(arr, PagePair), arr.shape[0], _sh(stream)))
 
+    def read_rows(self, layer: int, seqs, cell0, n_cells, k_out_dev, v_out_dev, stream=None, f16_rows: bool = False) -> None:
+        """Cells cell0[i] .. cell0[i] + n_cells[i] - 1 of sequence i as rows one after the other, f32 (or binary16 when f16_rows
+        is set) [sum n_cells][n_kv_head][head_dim]: the way back from append."""
+        seqs, ps = _i32(seqs)
+        cell0, pc = _i64(cell0)
+        n_cells, pn = _i32(n_cells)
+        assert seqs.size == cell0.size == n_cells.size
+        fn = lib.bkv_read_rows_f16 if f16_rows else lib.bkv_read_rows
+        check(fn(self.handle, layer, seqs.size, ps, pc, pn, _ptr(k_out_dev), _ptr(v_out_dev), _sh(stream)))
+
     def gather(self, layer: int, seq: int, cell0: int, n: int, stream=None):
         """Dequantised K and V rows as float32 arrays [n, n_kv, head_dim]."""
         shape = (n, self.desc.n_kv_head, self.desc.head_dim)

@@ -16,13 +16,13 @@ BENCH_HEADER_PATH = os.path.join(HERE, "..", "include", "breccia_kv_bench.h")
 
 OK, ERR_INVALID, ERR_RANGE, ERR_NO_PAGES, ERR_STATE, ERR_NO_DEVICE, ERR_HIP, ERR_NOMEM, ERR_TIMEOUT = range(9)
 STATUS_NAMES = ["OK", "INVALID", "RANGE", "NO_PAGES", "STATE", "NO_DEVICE", "HIP", "NOMEM", "TIMEOUT"]
-LAYOUT_F16, LAYOUT_Q8V, LAYOUT_I8H = 0, 1, 2
+LAYOUT_F16, LAYOUT_Q8V, LAYOUT_I8H, LAYOUT_F8P = 0, 1, 2, 3
 POOL_HOST_ONLY = 1
 MAX_BATCH = 64
 MAX_KV_HEAD = 16
 STATIC_WGS = 1024
 (STAGE_APPEND, STAGE_ATTN_SPLIT, STAGE_ATTN_MERGE, STAGE_PAGE_COPY, STAGE_PREFILL_ATTN, STAGE_APPEND_KPREP,
- STAGE_IDX_POOL, STAGE_IDX_SCORE, STAGE_TOPK, STAGE_PAGE_STAGE) = range(10)
+ STAGE_IDX_POOL, STAGE_IDX_SCORE, STAGE_TOPK, STAGE_PAGE_STAGE, STAGE_READ_ROWS) = range(11)
 
 
 class BkvError(RuntimeError):
@@ -134,6 +134,8 @@ _SIGNATURES = {
     "bkv_seq_evict": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp]),
     "bkv_seq_restore": (C.c_int, [_vp, _i32, _i32, _i32, _vp, _vp]),
     "bkv_gather": (C.c_int, [_vp, _i32, _i32, _i64, _i64, _vp, _vp, _vp]),
+    "bkv_read_rows": (C.c_int, [_vp, _i32, _i32, _pi32, _pi64, _pi32, _vp, _vp, _vp]),
+    "bkv_read_rows_f16": (C.c_int, [_vp, _i32, _i32, _pi32, _pi64, _pi32, _vp, _vp, _vp]),
 }
 
 _BENCH_SIGNATURES = {

@@ -54,8 +54,10 @@ typedef enum bkv_layout {
     BKV_LAYOUT_F16 = 0, /* f16 K and V: 2 B / element (reference default)                */
     BKV_LAYOUT_Q8V = 1, /* f16 K; V as q8_0 blocks [f32 scale][32 x i8] = 36 B / 32 values
                            (reference BRECCIA_KV_Q8V, shaders/qsa_kv_append.comp:38-44) */
-    BKV_LAYOUT_I8H = 2  /* int8 K and V, row = [head_dim x i8][head_dim/32 x f16 scale],
+    BKV_LAYOUT_I8H = 2, /* int8 K and V, row = [head_dim x i8][head_dim/32 x f16 scale],
                            34 B / 32 values (no reference counterpart)                   */
+    BKV_LAYOUT_F8P = 3  /* e4m3 K and V, one power of two as scale for each (page, kv head)
+                           of either: 1 B / value (no reference counterpart; below)      */
 } bkv_layout;
 
 enum {
@@ -229,6 +231,25 @@ bkv_status bkv_prefix_tier_stats(const bkv_pool *pool, int32_t *nodes_by_tier, u
  * tokens whose pages are on the device once the transfers are done. */
 bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_tokens,
                                int64_t *device_tokens);
+
+/* ---- BKV_LAYOUT_F8P -----------------------------------------------------------
+ * K and V in e4m3 (sign, 4 exponent bits of bias 7, 3 mantissa bits; no infinities, 0x7f and 0xff are NaN; largest 448), one
+ * power of two 2^e as scale for the 16 cells of a page, a kv head, of either side.  head_dim 256.  No reference counterpart.
+ *   e      the smallest of -32 .. 31 with which the largest finite magnitude among the unit's rows is at most 448 * 2^e
+ *          (31 where none is)
+ *   code   x * 2^-e rounded to nearest, ties to even; beyond +-448 the largest code; NaN for NaN and infinities
+ *   value  code * 2^e
+ * A write (bkv_append, _f16, _kprep; bkv_decode_step and step plans too) touches whole pages.  In a page that holds cells below
+ * the first one written those keep their values, under the scale of all of the page's rows -- exactly, but for values that a larger
+ * scale brings below 2^-6 * 2^e and which are rounded again, by at most 2^-10 * 2^e; cells behind the last one written are
+ * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, and two entries of
+ * one call must not write the same page (BKV_ERR_INVALID).  What a page holds depends on the rows written into it alone.
+ * A K page is n_kv_head units of 4096 bytes and a line of 128 with the exponents, int32 [kv head][K, V]; a V page n_kv_head units.
+ * In a unit, value d of cell c is at byte
+ *   K   1024 (c / 4) + 64 (8 (d / 128) + d / 4 % 8) + 16 (c % 4) + 4 (d / 32 % 4) + d % 4
+ *   V   1024 (c / 4) + 4 d + c % 4
+ * Exponents read from a page are brought into -32 .. 31.  A NaN in a row that a query attends makes NaN of what the query gets
+ * from it (K: the whole output row; V: its element), and of nothing else. */
 
 /* ---- hot path ---------------------------------------------------------------
  * bkv_append replaces Qsa::kv_append + shaders/qsa_kv_append.comp (qsa/mod.rs:
@@ -528,6 +549,16 @@ bkv_status bkv_seq_restore(bkv_pool *pool, int32_t seq, int32_t lp0, int32_t n,
 bkv_status bkv_gather(bkv_pool *pool, int32_t layer, int32_t seq, int64_t cell0, int64_t n,
                       float *k_out_dev, float *v_out_dev, void *stream);
 
+/* Rows read back, for code that wants them plain (a library's matrix product, a cache moved elsewhere): the way back from
+ * bkv_append / bkv_append_f16.  Cells cell0[i] .. cell0[i] + n_cells[i] - 1 of sequence seqs[i] as rows
+ * [sum n_cells][n_kv_head][head_dim], sequences concatenated in call order, one launch; f32, or binary16 (raw codes, the values
+ * rounded to nearest, ties to even).  Every layout.  The same sequence may appear several times, cells may overlap.  Error if a
+ * cell is outside the sequence's addressable ones or swapped out.  Outputs 16-byte aligned. */
+bkv_status bkv_read_rows(bkv_pool *pool, int32_t layer, int32_t n_seqs, const int32_t *seqs, const int64_t *cell0,
+                         const int32_t *n_cells, float *k_out_dev, float *v_out_dev, void *stream);
+bkv_status bkv_read_rows_f16(bkv_pool *pool, int32_t layer, int32_t n_seqs, const int32_t *seqs, const int64_t *cell0,
+                             const int32_t *n_cells, uint16_t *k_out_dev, uint16_t *v_out_dev, void *stream);
+
 /* How a decode-attention batch would be cut into work-groups on a device of n_cu compute units:
  * the planning step of bkv_decode_attn / bkv_decode_step / bkv_decode_attn_select alone, on the
  * host, nothing launched (no pool or device needed).  pos[n] as for those calls; sel_groups > 0
@@ -558,7 +589,8 @@ typedef enum bkv_stage {
     BKV_STAGE_IDX_SCORE = 7,
     BKV_STAGE_TOPK = 8,
     BKV_STAGE_PAGE_STAGE = 9,   /* gather / scatter of whole pages for swap and the prefix tiers */
-    BKV_STAGE_COUNT = 10
+    BKV_STAGE_READ_ROWS = 10,   /* rows read back (bkv_read_rows, and bkv_gather on BKV_LAYOUT_F8P) */
+    BKV_STAGE_COUNT = 11
 } bkv_stage;
 bkv_status bkv_timing_enable(bkv_pool *pool, int on);
 bkv_status bkv_timing_reset(bkv_pool *pool);
