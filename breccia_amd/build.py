@@ -29,7 +29,7 @@ HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-
 # The chunk attention kernel fills both halves of a wave's register file.  By default every matrix product of
 # such a kernel accumulates in the upper half, which the VALU cannot read; this option lets the register allocator
 # decide, product by product.
-FILE_FLAGS = {"prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "f8p_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+FILE_FLAGS = {"prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _hipcc() -> str:

@@ -92,7 +92,6 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
 typedef short tr_s4 __attribute__((__vector_size__(8)));  // what the transposing LDS read returns
 typedef __attribute__((address_space(3))) tr_s4* lds_tr_ptr;
-typedef const __attribute__((address_space(1))) uint8_t* page_ptr;  // said to be global memory: its address goes through integers
 
 // The chip is 8 dies (XCDs), each with an L2 of its own, and work-group i runs on die i % 8.
 // Every work-group of one (entry, kv head) unit walks the same K/V pages, so the dies are given
@@ -131,24 +130,6 @@ __device__ __forceinline__ float max_of(float a, float b) {
     asm("v_max_f32 %0, %0, %1" : "+v"(a) : "v"(b));
     return a;
 }
-
-// 16 bytes a lane straight into LDS: lane l's go to byte lds + 16 l.  Nothing but the vector-memory count says when they
-// have landed; each wave waits for its own ahead of the barrier that publishes them.
-__device__ __forceinline__ void load_to_lds(unsigned lds, page_ptr base, unsigned lane_off) {
-    // (the base came from a VALU instruction, which a vector-memory one must not follow closely: the copy is a scalar
-    // instruction, and the wait state that m0 wants)
-    uint64_t at;
-    // (m0 is reserved: the compiler keeps nothing there of its own accord, and warns that it would not; what it must not do is
-    // let a value that it puts there for an instruction of its own live across this)
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
-                 : "=&s"(at)
-                 : "s"(lds), "v"(lane_off), "s"(base)
-                 : "m0", "memory");
-#pragma clang diagnostic pop
-}
-__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // the maximum over the four lane groups; the swaps' neighbours and wait states stand in the same block
 __device__ __forceinline__ float max_over_groups(float x) {

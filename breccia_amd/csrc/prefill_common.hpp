@@ -73,6 +73,25 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t x, int i) {
     return (uint64_t)hi << 32 | lo;
 }
 
+typedef const __attribute__((address_space(1))) uint8_t* page_ptr;  // said to be global memory: its address goes through integers
+// 16 bytes a lane straight into LDS: lane l's go to byte lds + 16 l.  Nothing but the vector-memory count says when they
+// have landed; each wave waits for its own ahead of the barrier that publishes them.
+__device__ __forceinline__ void load_to_lds(unsigned lds, page_ptr base, unsigned lane_off) {
+    // (the base came from a VALU instruction, which a vector-memory one must not follow closely: the copy is a scalar
+    // instruction, and the wait state that m0 wants)
+    uint64_t at;
+    // (m0 is reserved: the compiler keeps nothing there of its own accord, and warns that it would not; what it must not do is
+    // let a value that it puts there for an instruction of its own live across this)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+                 : "=&s"(at)
+                 : "s"(lds), "v"(lane_off), "s"(base)
+                 : "m0", "memory");
+#pragma clang diagnostic pop
+}
+__device__ __forceinline__ void wait_for_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // The ranges of a cut call's rows put together (prefill_attn.hip).
 hipError_t launch_prefill_merge(bkv_pool* p, const PrefillSplitParams& kp, int32_t rows_per_wg, hipStream_t stream);
 // The chunk attention kernel of the e4m3 layout (f8p_chunk.hip), over `grid` work-groups of rows_per_wg rows; split: cut walks, which
