@@ -231,21 +231,25 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
         f8_u4 k[2][4], v[2][4];
         const auto load_k = [&](gptr base, int p, int i) { k[p][i] = *(const __attribute__((address_space(1))) f8_u4*)(base + 256 * i); };
         const auto load_v = [&](gptr base, int p, int m) { v[p][m] = *(const __attribute__((address_space(1))) f8_u4*)(base + 256 * m); };
-        const Pair first_ids = pair_ids(0);
-        Pair ids_v = pair_ids(2), ids_k = pair_ids(4);  // the pairs whose V and whose K is asked for next
+        Pair ids_0 = pair_ids(0), ids_1 = pair_ids(2), ids_2 = pair_ids(4);  // this pair, the next, the one after
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const gptr base = k_base(first_ids, p);
+            const gptr base = k_base(ids_0, p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) load_k(base, p, i);
         }
+        // With two tiles, a wave alone on its SIMD, V is asked for a step ahead.  With one the registers of a step's K become those
+        // of its V and back: the other wave's products cover what is left of the way (and 180 bytes a lane no longer spill).
+        constexpr bool kVAhead = TILES == 2;
+        if constexpr (kVAhead) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const gptr base = v_base(first_ids, p);
+            for (int p = 0; p < 2; ++p) {
+                const gptr base = v_base(ids_0, p);
 #pragma unroll
-            for (int m = 0; m < 4; ++m) load_v(base, p, m);
+                for (int m = 0; m < 4; ++m) load_v(base, p, m);
+            }
         }
-        f8_i2 ex[2] = {exps(first_ids, 0), exps(first_ids, 1)};
+        f8_i2 ex[2] = {exps(ids_0, 0), exps(ids_0, 1)};
 
         // ---- q as high and low parts: fragment f = 2 i + half of piece 4 i + g ----
         wait_for_loads();
@@ -376,7 +380,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
         for (int f = 0; f < 16; ++f) multiply_k(f);
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-            const gptr next = k_base(ids_v, p);
+            const gptr next = k_base(ids_1, p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) load_k(next, p, i);
         }
@@ -384,7 +388,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
 #pragma unroll
         for (int part = 0; part < 12; ++part) logits_part(part);
         move_reference(0);
-        ex[0] = exps(ids_v, 0), ex[1] = exps(ids_v, 1);
+        ex[0] = exps(ids_1, 0), ex[1] = exps(ids_1, 1);
 
         // A step: the next pair's scores with this one's weights between them, then this one's values with the next one's logits
         // between them.
@@ -401,7 +405,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                     }
             }
             const Pair ids_next = pair_ids(u + 6);
-            const f8_i2 ex_next[2] = {exps(ids_k, 0), exps(ids_k, 1)};
+            const f8_i2 ex_next[2] = {exps(ids_2, 0), exps(ids_2, 1)};
             float sum[TILES][2];
             f8_h8 ph[TILES], pl[TILES];
 #pragma unroll
@@ -426,12 +430,13 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                 }
             };
             {
-                const gptr next[2] = {k_base(ids_k, 0), k_base(ids_k, 1)};
+                const gptr next[2] = {kVAhead ? k_base(ids_2, 0) : v_base(ids_0, 0), kVAhead ? k_base(ids_2, 1) : v_base(ids_0, 1)};
 #pragma unroll
                 for (int f = 0; f < 16; ++f) {
                     multiply_k(f);
                     weights_part(f);
-                    if (f & 1) load_k(next[f >> 3], f >> 3, (f >> 1) & 3);
+                    if (kVAhead && (f & 1)) load_k(next[f >> 3], f >> 3, (f >> 1) & 3);
+                    if (!kVAhead && (f & 1)) load_v(next[(f >> 1) & 1], (f >> 1) & 1, f >> 2);
                 }
             }
 #pragma unroll
@@ -470,7 +475,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                 }
             }
             factors();
-            const gptr next_v[2] = {v_base(ids_v, 0), v_base(ids_v, 1)};
+            const gptr after[2] = {kVAhead ? v_base(ids_1, 0) : k_base(ids_2, 0), kVAhead ? v_base(ids_1, 1) : k_base(ids_2, 1)};
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -482,16 +487,36 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                     for (int t = 0; t < TILES; ++t) o[t][m][j] = f8_mfma(x, pl[t], o[t][m][j]);
                     logits_part(4 * m + j);
                 }
-                load_v(next_v[0], 0, m);
-                load_v(next_v[1], 1, m);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    if constexpr (kVAhead) load_v(after[p], p, m);
+                    else load_k(after[p], p, m);
+                }
             }
             move_reference(u + 2);
-            ids_v = ids_k, ids_k = ids_next;
+            ids_0 = ids_1, ids_1 = ids_2, ids_2 = ids_next;
             ex[0] = ex_next[0], ex[1] = ex_next[1];
         }
     }
 
     // ---- normalise, gate, store ----
+    // The gate's values of every row are asked for ahead of the rows' way through LDS, into the registers that q had: in batches of
+    // eight rows behind it they were a chain of trips to memory.
+    const bool gated = P.gate && !(SPLIT && cut);
+    const uint64_t gate_at = (uint64_t)(uintptr_t)P.gate + (uint64_t)((int64_t)out_row * P.gate_tok_stride + (int64_t)my_head * P.gate_head_stride) * 4;
+    f8_f4 gate[kRowsPerWave];
+    if (gated) {
+        if (P.gate_in_fours) {
+#pragma unroll
+            for (int r = 0; r < kRowsPerWave; ++r) gate[r] = *((in_f4)lane_value(gate_at, r) + lane);
+        } else {
+            typedef const __attribute__((address_space(1))) float* in_float;
+#pragma unroll
+            for (int r = 0; r < kRowsPerWave; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) gate[r][j] = ((in_float)lane_value(gate_at, r))[4 * lane + j];
+        }
+    }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
         if (__builtin_amdgcn_ballot_w64((poison[t][0] | poison[t][1]) != 0) != 0) {
@@ -533,32 +558,14 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
         }
     }
     const uint64_t out_at = (uint64_t)(uintptr_t)P.out + row_at;
-    const uint64_t gate_at = (uint64_t)(uintptr_t)P.gate + (uint64_t)((int64_t)out_row * P.gate_tok_stride + (int64_t)my_head * P.gate_head_stride) * 4;
-    constexpr int kAtOnce = 8;  // rows whose gate is asked for together
-    for (int r0 = 0; r0 < kRowsPerWave; r0 += kAtOnce) {
-        f8_f4 y[kAtOnce];
 #pragma unroll
-        for (int r = 0; r < kAtOnce; ++r) y[r] = staged(r0 + r);
-        if (P.gate) {
-            f8_f4 gv[kAtOnce];
-            if (P.gate_in_fours) {
+    for (int r = 0; r < kRowsPerWave; ++r) {
+        f8_f4 y = staged(r);
+        if (gated) {
 #pragma unroll
-                for (int r = 0; r < kAtOnce; ++r) gv[r] = *((in_f4)lane_value(gate_at, r0 + r) + lane);
-            } else {
-                typedef const __attribute__((address_space(1))) float* in_float;
-#pragma unroll
-                for (int r = 0; r < kAtOnce; ++r)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) gv[r][j] = ((in_float)lane_value(gate_at, r0 + r))[4 * lane + j];
-            }
-#pragma unroll
-            for (int r = 0; r < kAtOnce; ++r)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[r][j] *= sigmoid(gv[r][j]);
+            for (int j = 0; j < 4; ++j) y[j] *= sigmoid(gate[r][j]);
         }
-#pragma unroll
-        for (int r = 0; r < kAtOnce; ++r)
-            if (r0 + r < live_rows) *((out_f4)lane_value(out_at, r0 + r) + lane) = y[r];
+        if (r < live_rows) *((out_f4)lane_value(out_at, r) + lane) = y;
     }
 }
 
