@@ -1035,7 +1035,7 @@ static bkv_status decode_attn_common(bkv_pool* p, int32_t layer, int32_t n, cons
                                    : "decode_attn: %lld entries x %lld kv heads need more work-groups than the "
                                      "partial-result workspace holds (%lld); use smaller batches",
                          n, p->g.n_kv,
-                         attn_plan_limits(p->n_cu, ws_wgs, p->g.n_kv, n_q_head / p->g.n_kv).max_wgs));
+                         attn_plan_limits(p->n_cu, ws_wgs, p->g.n_kv, n_q_head / p->g.n_kv, p->g.layout).max_wgs));
     AttnArgs a;
     if (static_ws) {
         if (!attn_static_scratch(p->device, &a.ws_o, &a.ws_ml))
@@ -1104,7 +1104,7 @@ bkv_status bkv_attn_plan(int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int3
             return fail(BKV_ERR_RANGE, sfmt("attn_plan: position %lld of entry %lld", pos[i], i));
         b.pos[i] = (int32_t)pos[i];
     }
-    const AttnPlanLimits lim = attn_plan_limits(n_cu, kMaxWgs, n_kv_head, n_q_head / n_kv_head);
+    const AttnPlanLimits lim = attn_plan_limits(n_cu, kMaxWgs, n_kv_head, n_q_head / n_kv_head, BKV_LAYOUT_F16);
     const int32_t total = plan_attn_ranges(lim, 16, sel_groups, b);
     if (total < 0)
         return fail(BKV_ERR_INVALID, sfmt("attn_plan: %lld entries x %lld kv heads need more work-groups than "
@@ -1218,7 +1218,7 @@ bkv_status bkv_step_plan_create(bkv_pool* p, int32_t n, const int32_t* seqs, con
     bkv_status st = need_device(p);
     if (st != BKV_OK) return st;
     const int32_t group = n_q_head / p->g.n_kv;
-    const AttnPlanLimits lim = attn_plan_limits(p->n_cu, p->max_wgs, p->g.n_kv, group);
+    const AttnPlanLimits lim = attn_plan_limits(p->n_cu, p->max_wgs, p->g.n_kv, group, p->g.layout);
     if (plan_attn_ranges(lim, p->g.page_cells, 0, host.b) < 0)
         return fail(BKV_ERR_INVALID, sfmt("step_plan_create: %lld entries x %lld kv heads need more work-groups "
                                           "than the partial-result workspace holds (%lld)", n, p->g.n_kv,

@@ -278,7 +278,7 @@ hipError_t launch_step_advance(StepDesc* d, const AttnPlanLimits& lim, int32_t p
 // Fills wg_base/splits/pps from row/pos (attn_plan.hpp); returns the total work-group count, -1
 // when the batch cannot be cut into as few work-groups as the workspace holds.  sel_groups > 0:
 // every entry is planned for that many groups of four selected blocks instead of its pages.
-AttnPlanLimits attn_plan_limits(int32_t n_cu, int32_t max_wgs, int32_t n_kv, int32_t group);
+AttnPlanLimits attn_plan_limits(int32_t n_cu, int32_t max_wgs, int32_t n_kv, int32_t group, int32_t layout);
 int32_t plan_attn(const bkv_pool* p, int32_t n_q_head, AttnBatch& b, int32_t sel_groups = 0, int32_t max_wgs = 0);
 // The static device scratch of bkv_decode_attn_static: looked up once per device (which must be
 // the current one) at pool creation; false from the accessor when that has not happened.

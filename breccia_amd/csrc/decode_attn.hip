@@ -187,10 +187,11 @@ __global__ __launch_bounds__(64 * kMergeWaves) void decode_attn_merge_kernel(con
 
 // The limits a plan of this pool geometry works under.  The partial-result workspace holds
 // max_wgs x 8 head rows and a work-group writes `group` of them.
-AttnPlanLimits attn_plan_limits(int32_t n_cu, int32_t max_wgs, int32_t n_kv, int32_t group) {
+AttnPlanLimits attn_plan_limits(int32_t n_cu, int32_t max_wgs, int32_t n_kv, int32_t group, int32_t layout) {
     AttnPlanLimits lim;
     lim.per_page = n_kv;
-    lim.gran = kWaves;
+    // (e4m3: a wave takes two pages at a time; a range of one is no sooner done, and there are twice as many to merge)
+    lim.gran = layout == BKV_LAYOUT_F8P ? 2 * kWaves : kWaves;
     // All work-groups should be resident at once (one generation): a handful of left-over
     // work-groups would run alone after the rest and double the kernel's time.  Two work-groups
     // fit a compute unit (registers and LDS of the kernels).
@@ -201,7 +202,7 @@ AttnPlanLimits attn_plan_limits(int32_t n_cu, int32_t max_wgs, int32_t n_kv, int
 
 int32_t plan_attn(const bkv_pool* p, int32_t n_q_head, AttnBatch& b, int32_t sel_groups, int32_t max_wgs) {
     const AttnPlanLimits lim =
-        attn_plan_limits(p->n_cu, max_wgs > 0 ? max_wgs : p->max_wgs, p->g.n_kv, n_q_head / p->g.n_kv);
+        attn_plan_limits(p->n_cu, max_wgs > 0 ? max_wgs : p->max_wgs, p->g.n_kv, n_q_head / p->g.n_kv, p->g.layout);
     return plan_attn_ranges(lim, kPage, sel_groups, b);
 }
 
@@ -287,7 +288,7 @@ hipError_t launch_decode_attn(bkv_pool* p, int32_t layer, const AttnBatch& b, co
     // the events ride on the dispatch
     hipEvent_t ev_start = nullptr, ev_stop = nullptr;
     if (a.timed) (void)timer_dispatch_events(p, BKV_STAGE_ATTN_SPLIT, &ev_start, &ev_stop);
-    hipError_t err = p->g.layout == BKV_LAYOUT_F8P ? launch_decode_attn_f8p(kp, b, sel, total, stream, ev_start, ev_stop)
+    hipError_t err = p->g.layout == BKV_LAYOUT_F8P ? launch_decode_attn_f8p(kp, b, p->g.n_layers, sel, total, stream, ev_start, ev_stop)
                                                    : launch_decode_attn_mfma(kp, b, p->g.layout, step, sel, total, stream, ev_start, ev_stop);
     if (err != hipSuccess) return err;
     MergeParams mp;

@@ -155,7 +155,7 @@ __device__ __forceinline__ bool block_cell_live(uint32_t id, int r, int pos) {
 hipError_t launch_decode_attn_mfma(const AttnKernelParams& kp, const AttnBatch& b, int layout, bool step, bool sel, int32_t total,
                                    hipStream_t stream, hipEvent_t start = nullptr, hipEvent_t stop = nullptr);
 // The same of the e4m3 layout (f8p_decode.hip); a step's rows have been appended by a launch of their own.
-hipError_t launch_decode_attn_f8p(const AttnKernelParams& kp, const AttnBatch& b, bool sel, int32_t total, hipStream_t stream, hipEvent_t start,
-                                  hipEvent_t stop);
+hipError_t launch_decode_attn_f8p(const AttnKernelParams& kp, const AttnBatch& b, int32_t n_layers, bool sel, int32_t total, hipStream_t stream,
+                                  hipEvent_t start, hipEvent_t stop);
 
 }  // namespace bkv

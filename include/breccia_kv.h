@@ -559,7 +559,8 @@ bkv_status bkv_read_rows(bkv_pool *pool, int32_t layer, int32_t n_seqs, const in
 bkv_status bkv_read_rows_f16(bkv_pool *pool, int32_t layer, int32_t n_seqs, const int32_t *seqs, const int64_t *cell0,
                              const int32_t *n_cells, uint16_t *k_out_dev, uint16_t *v_out_dev, void *stream);
 
-/* How a decode-attention batch would be cut into work-groups on a device of n_cu compute units:
+/* How a decode-attention batch would be cut into work-groups on a device of n_cu compute units (on a
+ * BKV_LAYOUT_F8P pool ranges are multiples of eight pages instead of four):
  * the planning step of bkv_decode_attn / bkv_decode_step / bkv_decode_attn_select alone, on the
  * host, nothing launched (no pool or device needed).  pos[n] as for those calls; sel_groups > 0
  * plans every entry for that many groups of four listed blocks (a selection list of
