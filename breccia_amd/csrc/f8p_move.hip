@@ -1,9 +1,12 @@
 // Rows into and out of pools in the e4m3 layout (f8p.hpp), for gfx950.
 //
-// Written rows join a page under one scale with the rows below them that it holds already.  So a work-group has a whole
-// (page, kv head), K and V: it holds all 16 rows of both in registers, 16 + 16 values a thread, agrees on the two largest
-// magnitudes, and writes all codes of the page.  Rows behind the last one written are cleared: what a page holds follows from
-// the rows written into it, whoever had it before.
+// Written rows join a page under one scale with the rows below them that it holds already.  So a work-group has a whole unit,
+// K or V of a (page, kv head): it holds all 16 rows in registers, 16 values a thread, agrees on the largest magnitude, and
+// writes all codes.  Rows behind the last one written are cleared: what a page holds follows from the rows written into it,
+// whoever had it before.  (K and V in one work-group: five ragged chunks of 2073 rows at n_kv = 4 9.5 us, apart 8.7.)
+//
+// Everything here moves bytes.  Small calls take what a launch and two dependent trips to memory take, 3.5 us; reading back
+// 131072 cells as binary16, 402 MB, takes 67 us, 6.0 TB/s, what a copy reaches here.
 #include <algorithm>
 #include <type_traits>
 
@@ -64,54 +67,46 @@ struct F8Share {
 };
 __device__ __forceinline__ void transpose4x4(const unsigned (&w)[4], unsigned (&t)[4]) { transpose4x4_bytes(w, t); }
 
-// The values of a page that lie in registers, coded and stored.  k[u]: elements k_col + 32 u ..; v[i]: row v_row + i.
-// Rows below `kept` are in the page and come from old_k / old_v (loaded by the caller, under their old scales), rows from `end`
-// on are cleared.
+// One half (K or V) of a unit that lies in registers, x[u]: K's elements k_col + 32 u .., V's row v_row + u, coded and stored.
+// Rows below `kept` are in the page and come from `old` (loaded by the caller) under their old scale, rows from `end` on are
+// cleared.
 struct F8Old {
-    v4u k, v;
-    int ek, ev;
+    v4u w;
+    int e;
 };
-__device__ __forceinline__ void store_page(const F8Share& at, float (&k)[4][4], float (&v)[4][4], int kept, int end, const F8Old& old, float* red,
-                                           uint8_t* kunit, uint8_t* vunit, int32_t* line, int tid) {
-    float ka = 0.0f, va = 0.0f;
+// First the page's rows as they are to be, and the wave's largest magnitude to red[wave]; behind a barrier, the codes.
+template <bool V>
+__device__ __forceinline__ void settle_rows(const F8Share& at, float (&x)[4][4], int kept, int end, const F8Old& old, float* red, int tid) {
+    const auto row = [&](int u) { return V ? at.v_row + u : at.k_row; };
     if (kept > 0) {
-        const float ks = exp2_int(old.ek), vs = exp2_int(old.ev);
-        if (at.k_row < kept) {
+        const float scale = exp2_int(old.e);
+        unsigned in[4] = {old.w.x, old.w.y, old.w.z, old.w.w}, rows[4];
+        if constexpr (V) transpose4x4(in, rows);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) f8p_values4(old.k[u], ks, k[u]);
-        }
-        unsigned cols[4] = {old.v.x, old.v.y, old.v.z, old.v.w}, rows[4];
-        transpose4x4(cols, rows);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at.v_row + i < kept) f8p_values4(rows[i], vs, v[i]);
+        for (int u = 0; u < 4; ++u)
+            if (row(u) < kept) f8p_values4(V ? rows[u] : in[u], scale, x[u]);
     }
+    float top = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (at.k_row >= end) k[u][i] = 0.0f;
-            if (at.v_row + u >= end) v[u][i] = 0.0f;
-            ka = amax_finite(ka, k[u][i]);
-            va = amax_finite(va, v[u][i]);
+            if (row(u) >= end) x[u][i] = 0.0f;
+            top = amax_finite(top, x[u][i]);
         }
-    ka = wave_max_of(ka);
-    va = wave_max_of(va);
-    if ((tid & 63) == 0) red[(tid >> 6) * 2] = ka, red[(tid >> 6) * 2 + 1] = va;
-    __syncthreads();
-    const int ek = f8p_exponent(fmaxf(fmaxf(red[0], red[2]), fmaxf(red[4], red[6])));
-    const int ev = f8p_exponent(fmaxf(fmaxf(red[1], red[3]), fmaxf(red[5], red[7])));
-    const float ki = exp2_int(-ek), vi = exp2_int(-ev);
-    v4u ko;
+    top = wave_max_of(top);
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+}
+template <bool V>
+__device__ __forceinline__ void store_codes(const F8Share& at, const float (&x)[4][4], const float* red, uint8_t* unit, int32_t* exponent, int tid) {
+    const int e = f8p_exponent(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+    const float by = exp2_int(-e);
+    unsigned codes[4], out[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) ko[u] = f8p_codes4(k[u], ki);
-    unsigned rows[4], cols[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) rows[i] = f8p_codes4(v[i], vi);
-    transpose4x4(rows, cols);
-    *reinterpret_cast<v4u*>(kunit + at.k_at) = ko;
-    *reinterpret_cast<v4u*>(vunit + at.v_at) = v4u{cols[0], cols[1], cols[2], cols[3]};
-    if (tid == 0) line[0] = ek, line[1] = ev;
+    for (int u = 0; u < 4; ++u) out[u] = codes[u] = f8p_codes4(x[u], by);
+    if constexpr (V) transpose4x4(codes, out);
+    *reinterpret_cast<v4u*>(unit + (V ? at.v_at : at.k_at)) = v4u{out[0], out[1], out[2], out[3]};
+    if (tid == 0) *exponent = e;
 }
 
 struct F8Target {
@@ -127,13 +122,23 @@ __device__ __forceinline__ F8Target target_of(const F8MoveGeom& g, uint8_t* kpoo
     t.line = reinterpret_cast<int32_t*>(kp + (size_t)g.n_kv * kF8Unit) + 2 * kvh;
     return t;
 }
+template <bool V>
 __device__ __forceinline__ F8Old old_of(const F8Target& t, const F8Share& at) {
-    F8Old o;
-    o.k = *reinterpret_cast<const v4u*>(t.kunit + at.k_at);
-    o.v = *reinterpret_cast<const v4u*>(t.vunit + at.v_at);
-    o.ek = f8p_exponent_read(t.line[0]);
-    o.ev = f8p_exponent_read(t.line[1]);
-    return o;
+    return F8Old{*reinterpret_cast<const v4u*>(V ? t.vunit + at.v_at : t.kunit + at.k_at), f8p_exponent_read(t.line[V])};
+}
+
+// Which of a launch's work a work-group has: (page of the entry, kv head, K or V), both halves of a (page, kv head) side by side,
+// in turns so that the dies, which have every eighth work-group, get as much of K as of V.
+struct F8Work {
+    int at_page, kvh;
+    bool v;
+};
+__device__ __forceinline__ F8Work work_of(int x, int n_kv) {
+    F8Work w;
+    w.v = ((x ^ (x >> 3)) & 1) != 0;
+    w.at_page = (x >> 1) / n_kv;
+    w.kvh = (x >> 1) - w.at_page * n_kv;
+    return w;
 }
 
 // One work-group per (page of an entry, kv head): grid (pages of the longest entry x kv heads, entries).
@@ -150,38 +155,57 @@ struct F8DescBatch {
 };
 __device__ __forceinline__ F8Rows rows_of(const F8DescBatch& b, int s) { return F8Rows{b.bd->row[s], b.bd->pos[s], 1, s}; }
 
+// The rows of a work-group's page: where they come from, which of them the call writes.
+struct F8Span {
+    int page, kept, end;
+};
+__device__ __forceinline__ F8Span span_of(const F8Rows& r, int at_page) {
+    F8Span s;
+    s.page = r.pos0 / kF8Page + at_page;
+    s.kept = max(r.pos0 - s.page * kF8Page, 0);
+    s.end = min(r.pos0 + r.n_tok - s.page * kF8Page, kF8Page);
+    return s;
+}
+// (rows outside of the call's are clamped to it and dropped: no branch around a load)
+__device__ __forceinline__ size_t source_of(const F8Rows& r, const F8Span& s, int n_kv, int kvh, int row, int col) {
+    const int tok = min(max(s.page * kF8Page + row - r.pos0, 0), r.n_tok - 1);
+    return (((size_t)r.src0 + (size_t)tok) * (size_t)n_kv + (size_t)kvh) * kF8Hd + (size_t)col;
+}
+
+template <bool V, typename SrcT>
+__device__ __forceinline__ void append_unit(const F8Rows& r, const F8Span& s, int n_kv, int kvh, const F8Target& t, const SrcT* __restrict__ src,
+                                            float* red) {
+    const int tid = threadIdx.x;
+    const F8Share at(tid);
+    float x[4][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        load4(src + (V ? source_of(r, s, n_kv, kvh, at.v_row + u, at.v_col) : source_of(r, s, n_kv, kvh, at.k_row, at.k_col + 32 * u)), x[u]);
+    F8Old old{};
+    if (s.kept > 0) old = old_of<V>(t, at);
+    settle_rows<V>(at, x, s.kept, s.end, old, red, tid);
+    __syncthreads();
+    store_codes<V>(at, x, red, V ? t.vunit : t.kunit, t.line + V, tid);
+}
 template <typename SrcT, typename Batch>
 __global__ __launch_bounds__(kBlock) void append_f8p_kernel(Batch b, F8MoveGeom g, uint8_t* __restrict__ kpool, uint8_t* __restrict__ vpool,
                                                             const int32_t* __restrict__ tables, const SrcT* __restrict__ ks,
                                                             const SrcT* __restrict__ vs) {
-    __shared__ float red[2 * kF8Waves];
+    __shared__ float red[kF8Waves];
     const F8Rows r = rows_of(b, blockIdx.y);
-    const int first_page = r.pos0 / kF8Page;
-    const int at_page = (int)blockIdx.x / g.n_kv, kvh = (int)blockIdx.x - at_page * g.n_kv;
-    const int page = first_page + at_page;
-    if (r.n_tok == 0 || page > (r.pos0 + r.n_tok - 1) / kF8Page) return;
-    const int tid = threadIdx.x;
-    const F8Share at(tid);
-    const F8Target t = target_of(g, kpool, vpool, tables, r.row, page, kvh);
-    const int kept = max(r.pos0 - page * kF8Page, 0), end = min(r.pos0 + r.n_tok - page * kF8Page, kF8Page);
-    // rows outside of the call's are clamped to it and dropped: no branch around a load
-    const auto src = [&](int row, int col) -> size_t {
-        const int tok = min(max(page * kF8Page + row - r.pos0, 0), r.n_tok - 1);
-        return (((size_t)r.src0 + (size_t)tok) * (size_t)g.n_kv + (size_t)kvh) * kF8Hd + (size_t)col;
-    };
-    float k[4][4], v[4][4];
-    const size_t k0 = src(at.k_row, at.k_col);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load4(ks + k0 + 32 * u, k[u]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load4(vs + src(at.v_row + i, at.v_col), v[i]);
-    F8Old old{};
-    if (kept > 0) old = old_of(t, at);
-    store_page(at, k, v, kept, end, old, red, t.kunit, t.vunit, t.line, tid);
+    const F8Work w = work_of(blockIdx.x, g.n_kv);
+    const F8Span s = span_of(r, w.at_page);
+    if (s.end <= 0 || r.n_tok == 0) return;
+    const F8Target t = target_of(g, kpool, vpool, tables, r.row, s.page, w.kvh);
+    if (w.v) append_unit<true>(r, s, g.n_kv, w.kvh, t, vs, red);
+    else append_unit<false>(r, s, g.n_kv, w.kvh, t, ks, red);
 }
 
-// The same with K through RMSNorm and the rotary first; stages and arithmetic as in append_kprep_kernel (kv_move.hip), which this
-// layout shares but for the unit of work, a (page, kv head).
+// The same with K through RMSNorm and the rotary first; arithmetic as in append_kprep_kernel (kv_move.hip).  A work-group has both
+// halves of a (page, kv head): V arrives, is coded and stored while one wave adds up K's squares, one after the other as the sum
+// is defined.  Eight work-groups a compute unit, as many as LDS and threads let be there, hide what they can of that chain
+// (registers are kept to that: 86 of them and five work-groups cost two prompts of 8191 tokens 3 us).  Those, 84 MB, take 21.7 us;
+// without the sums, the products and the rotary, 17 us.
 struct F8Prep {
     const float* gamma;
     const float* table;
@@ -190,73 +214,66 @@ struct F8Prep {
     int32_t n_rot, max_pos;
 };
 constexpr int kPrepStride = kF8Hd + 4;
-__global__ __launch_bounds__(kBlock) void append_kprep_f8p_kernel(AppendBatch b, F8MoveGeom g, F8Prep kp, uint8_t* __restrict__ kpool,
-                                                                  uint8_t* __restrict__ vpool, const int32_t* __restrict__ tables,
-                                                                  const float* __restrict__ ks, const float* __restrict__ vs) {
+__global__ __launch_bounds__(kBlock, 8) void append_kprep_f8p_kernel(AppendBatch b, F8MoveGeom g, F8Prep kp, uint8_t* __restrict__ kpool,
+                                                                     uint8_t* __restrict__ vpool, const int32_t* __restrict__ tables,
+                                                                     const float* __restrict__ ks, const float* __restrict__ vs) {
 #pragma clang fp contract(off)
-    __shared__ float red[2 * kF8Waves];
+    __shared__ float red_v[kF8Waves], red_k[kF8Waves];
     __shared__ __attribute__((aligned(16))) float rows_s[kF8Page * kPrepStride];
     __shared__ double inv_s[kF8Page];
-    __shared__ int pos_s[kF8Page];
     const F8Rows r = rows_of(b, blockIdx.y);
-    const int first_page = r.pos0 / kF8Page;
     const int at_page = (int)blockIdx.x / g.n_kv, kvh = (int)blockIdx.x - at_page * g.n_kv;
-    const int page = first_page + at_page;
-    if (r.n_tok == 0 || page > (r.pos0 + r.n_tok - 1) / kF8Page) return;
+    const F8Span s = span_of(r, at_page);
+    if (s.end <= 0 || r.n_tok == 0) return;
     const int tid = threadIdx.x;
     const F8Share at(tid);
-    const F8Target t = target_of(g, kpool, vpool, tables, r.row, page, kvh);
-    const int kept = max(r.pos0 - page * kF8Page, 0), end = min(r.pos0 + r.n_tok - page * kF8Page, kF8Page);
-    const auto src = [&](int row, int col) -> size_t {
-        const int tok = min(max(page * kF8Page + row - r.pos0, 0), r.n_tok - 1);
-        return (((size_t)r.src0 + (size_t)tok) * (size_t)g.n_kv + (size_t)kvh) * kF8Hd + (size_t)col;
-    };
+    const F8Target t = target_of(g, kpool, vpool, tables, r.row, s.page, kvh);
     float v[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float x[4];
-        load4(ks + src(at.v_row + i, at.v_col), x);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) rows_s[(at.v_row + i) * kPrepStride + at.v_col + j] = x[j];
+        load4(ks + source_of(r, s, g.n_kv, kvh, at.v_row + i, at.v_col), x);
+        *reinterpret_cast<float4*>(rows_s + (at.v_row + i) * kPrepStride + at.v_col) = make_float4(x[0], x[1], x[2], x[3]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) load4(vs + src(at.v_row + i, at.v_col), v[i]);
+    for (int i = 0; i < 4; ++i) load4(vs + source_of(r, s, g.n_kv, kvh, at.v_row + i, at.v_col), v[i]);
     const float gamma = kp.gamma[tid];
     F8Old old{};
-    if (kept > 0) old = old_of(t, at);
-    if (tid >= 64 && tid < 64 + kF8Page) {
-        // (clamped to the call's cells: positions need not cover others)
-        const int cell = min(max(page * kF8Page + tid - 64, r.pos0), r.pos0 + r.n_tok - 1);
-        const int64_t pos = kp.positions ? (int64_t)kp.positions[cell] : (int64_t)cell;
-        pos_s[tid - 64] = (int)(pos < 0 ? 0 : (pos > kp.max_pos - 1 ? kp.max_pos - 1 : pos));
-    }
+    if (s.kept > 0) old = old_of<true>(t, at);
     __syncthreads();
-    if (tid < kF8Page) {
-        double ss = 0.0;  // in element order
-#pragma unroll 8
+    // (one wave of the four, another in the next work-group: a compute unit's would all wait for one SIMD: 0.7 us of the prompts')
+    const int sum_row = (tid ^ (int)(blockIdx.x << 6)) & (kBlock - 1);
+    if (sum_row < kF8Page) {
+        double ss = 0.0;  // in element order; a product of two floats is exact, fused it is the same sum
+#pragma unroll 4
         for (int i = 0; i < kF8Hd; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(rows_s + tid * kPrepStride + i);
-            ss += (double)x.x * (double)x.x;
-            ss += (double)x.y * (double)x.y;
-            ss += (double)x.z * (double)x.z;
-            ss += (double)x.w * (double)x.w;
+            const float4 x = *reinterpret_cast<const float4*>(rows_s + sum_row * kPrepStride + i);
+            ss = __builtin_fma((double)x.x, (double)x.x, ss);
+            ss = __builtin_fma((double)x.y, (double)x.y, ss);
+            ss = __builtin_fma((double)x.z, (double)x.z, ss);
+            ss = __builtin_fma((double)x.w, (double)x.w, ss);
         }
-        inv_s[tid] = 1.0 / sqrt(ss / (double)kF8Hd + (double)kp.eps);
+        inv_s[sum_row] = 1.0 / sqrt(ss / (double)kF8Hd + (double)kp.eps);
     }
+    settle_rows<true>(at, v, s.kept, s.end, old, red_v, tid);
     __syncthreads();
-#pragma unroll
+    store_codes<true>(at, v, red_v, t.vunit, t.line + 1, tid);
+#pragma unroll 4
     for (int row = 0; row < kF8Page; ++row) {
         float* d = rows_s + row * kPrepStride + tid;
         *d = (float)((double)*d * inv_s[row] * (double)gamma);
     }
     __syncthreads();
-    const int half = kp.n_rot / 2;
-    for (int idx = tid; idx < kF8Page * half; idx += kBlock) {
-        const int row = idx & (kF8Page - 1), j = idx / kF8Page;
-        const float2 cs = reinterpret_cast<const float2*>(kp.table)[(size_t)pos_s[row] * half + j];
-        float* d = rows_s + row * kPrepStride;
-        const double x = (double)d[j], y = (double)d[j + half], c = (double)cs.x, s = (double)cs.y;
-        const double xc = x * c, ys = y * s, xs = x * s, yc = y * c;
+    // the rotary: pairs tid / 16 + 16 i of row tid % 16 (clamped to the call's cells: positions need not cover others)
+    const int half = kp.n_rot / 2, rot_row = tid & (kF8Page - 1);
+    const int cell = min(max(s.page * kF8Page + rot_row, r.pos0), r.pos0 + r.n_tok - 1);
+    const int pos = min(max(kp.positions ? kp.positions[cell] : cell, 0), kp.max_pos - 1);
+    const float2* const factors = reinterpret_cast<const float2*>(kp.table) + (size_t)pos * half;
+    float* const d = rows_s + rot_row * kPrepStride;
+    for (int j = tid / kF8Page; j < half; j += kBlock / kF8Page) {
+        const float2 cs = factors[j];
+        const double x = (double)d[j], y = (double)d[j + half], c = (double)cs.x, si = (double)cs.y;
+        const double xc = x * c, ys = y * si, xs = x * si, yc = y * c;
         d[j] = (float)(xc - ys);
         d[j + half] = (float)(xs + yc);
     }
@@ -267,7 +284,10 @@ __global__ __launch_bounds__(kBlock) void append_kprep_f8p_kernel(AppendBatch b,
         const float4 x = *reinterpret_cast<const float4*>(rows_s + at.k_row * kPrepStride + at.k_col + 32 * u);
         k[u][0] = x.x, k[u][1] = x.y, k[u][2] = x.z, k[u][3] = x.w;
     }
-    store_page(at, k, v, kept, end, old, red, t.kunit, t.vunit, t.line, tid);
+    if (s.kept > 0) old = old_of<false>(t, at);
+    settle_rows<false>(at, k, s.kept, s.end, old, red_k, tid);
+    __syncthreads();
+    store_codes<false>(at, k, red_k, t.kunit, t.line, tid);
 }
 
 // ---- rows read back -----------------------------------------------------------------------------------
@@ -282,6 +302,16 @@ __device__ __forceinline__ void put4(uint16_t* p, const float (&x)[4]) {
     __builtin_nontemporal_store(__builtin_bit_cast(v2u, h), reinterpret_cast<v2u*>(p));
 }
 
+__device__ __forceinline__ void put8(uint16_t* p, const float (&x)[8]) {
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    h8 h;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = (_Float16)x[i];
+    __builtin_nontemporal_store(__builtin_bit_cast(v4u, h), reinterpret_cast<v4u*>(p));
+}
+// the neighbour's (lane ^ 1) value
+__device__ __forceinline__ unsigned of_neighbour(unsigned x) { return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true); }
+
 // e4m3 pools: a work-group per (page, kv head), shares as on the way in.
 template <typename DstT, typename Batch>
 __global__ __launch_bounds__(kBlock) void read_rows_f8p_kernel(Batch b, F8MoveGeom g, const uint8_t* __restrict__ kpool,
@@ -294,28 +324,48 @@ __global__ __launch_bounds__(kBlock) void read_rows_f8p_kernel(Batch b, F8MoveGe
     if (r.n_tok == 0 || page > (r.pos0 + r.n_tok - 1) / kF8Page) return;
     const F8Share at(threadIdx.x);
     const F8Target t = target_of(g, const_cast<uint8_t*>(kpool), const_cast<uint8_t*>(vpool), tables, r.row, page, kvh);
-    const F8Old x = old_of(t, at);
+    const F8Old k = old_of<false>(t, at), v = old_of<true>(t, at);
     const auto live = [&](int row) { return page * kF8Page + row >= r.pos0 && page * kF8Page + row < r.pos0 + r.n_tok; };
     const auto dst = [&](int row, int col) -> size_t {
         return (((size_t)r.src0 + (size_t)(page * kF8Page + row - r.pos0)) * (size_t)g.n_kv + (size_t)kvh) * kF8Hd + (size_t)col;
     };
-    const float ks = exp2_int(x.ek), vs = exp2_int(x.ev);
-    if (live(at.k_row)) {
-        const size_t k0 = dst(at.k_row, at.k_col);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            float y[4];
-            f8p_values4(x.k[u], ks, y);
-            put4(ko + k0 + 32 * u, y);
-        }
-    }
-    unsigned cols[4] = {x.v.x, x.v.y, x.v.z, x.v.w}, rows[4];
+    const float ks = exp2_int(k.e), vs = exp2_int(v.e);
+    unsigned cols[4] = {v.w.x, v.w.y, v.w.z, v.w.w}, rows[4];
     transpose4x4(cols, rows);
+    if constexpr (std::is_same<DstT, uint16_t>::value) {
+        // Two lanes have neighbouring fours: the even one takes both fours of the even dwords, the odd one of the odd dwords, and
+        // stores are 16 bytes a lane, whole 128-byte lines an instruction.
+        const bool odd = threadIdx.x & 1;
+        const auto store = [&](unsigned even_w, unsigned odd_w, float scale, DstT* to) {
+            const unsigned mine = odd ? odd_w : even_w, theirs = of_neighbour(odd ? even_w : odd_w);
+            float lo[4], hi[4];
+            f8p_values4(odd ? theirs : mine, scale, lo);
+            f8p_values4(odd ? mine : theirs, scale, hi);
+            const float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (to) put8(to, y);
+        };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float y[4];
-        f8p_values4(rows[i], vs, y);
-        if (live(at.v_row + i)) put4(vo + dst(at.v_row + i, at.v_col), y);
+        for (int i = 0; i < 2; ++i)
+            store(k.w[2 * i], k.w[2 * i + 1], ks, live(at.k_row) ? ko + dst(at.k_row, at.k_col - 4 * odd + 32 * (2 * i + odd)) : nullptr);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            store(rows[2 * i], rows[2 * i + 1], vs, live(at.v_row + 2 * i + odd) ? vo + dst(at.v_row + 2 * i + odd, at.v_col - 4 * odd) : nullptr);
+    } else {
+        if (live(at.k_row)) {
+            const size_t k0 = dst(at.k_row, at.k_col);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float y[4];
+                f8p_values4(k.w[u], ks, y);
+                put4(ko + k0 + 32 * u, y);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float y[4];
+            f8p_values4(rows[i], vs, y);
+            if (live(at.v_row + i)) put4(vo + dst(at.v_row + i, at.v_col), y);
+        }
     }
 }
 
@@ -392,7 +442,7 @@ void with_batch(const AppendBatch& b, F f) {
 
 hipError_t launch_append_f8p(bkv_pool* p, int32_t layer, const AppendBatch& b, const void* k, const void* v, bool src_is_f16,
                              hipStream_t stream) {
-    const dim3 grid(pages_of(b) * (unsigned)p->g.n_kv, (unsigned)b.n);
+    const dim3 grid(pages_of(b) * (unsigned)p->g.n_kv * 2, (unsigned)b.n);
     with_batch(b, [&](const auto& batch) {
         using Batch = std::decay_t<decltype(batch)>;
         const auto launch = [&](auto kernel, auto ks, auto vs) {
@@ -407,7 +457,7 @@ hipError_t launch_append_f8p(bkv_pool* p, int32_t layer, const AppendBatch& b, c
 
 hipError_t launch_append_f8p_desc(bkv_pool* p, int32_t layer, const AttnBatch* desc, int32_t n, const float* k, const float* v,
                                   hipStream_t stream) {
-    hipLaunchKernelGGL((append_f8p_kernel<float, F8DescBatch>), dim3((unsigned)p->g.n_kv, (unsigned)n), dim3(kBlock), 0, stream,
+    hipLaunchKernelGGL((append_f8p_kernel<float, F8DescBatch>), dim3((unsigned)p->g.n_kv * 2, (unsigned)n), dim3(kBlock), 0, stream,
                        F8DescBatch{desc}, f8_geom(p), p->k_layer[(size_t)layer], p->v_layer[(size_t)layer], (const int32_t*)p->table_dev, k, v);
     return hipGetLastError();
 }
