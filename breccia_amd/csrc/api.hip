@@ -871,6 +871,10 @@ static bkv_status build_append_batch(bkv_pool* p, int32_t layer, int32_t n_seqs,
                                                       "which this layout writes as a whole; one entry, or two calls", j, i, seqs[i]));
     }
     b.n = n_seqs;
+    // (a launch has fewer than 2^32 threads along an axis, 256 of them for each page, kv head and side)
+    if (p->g.layout == BKV_LAYOUT_F8P && ((int64_t)max_tok / p->g.page_cells + 2) * p->g.n_kv * 512 >= (int64_t)1 << 32)
+        return fail(BKV_ERR_INVALID, sfmt("append: %lld rows of one sequence in a call are more than a launch takes at %lld kv heads", max_tok,
+                                          p->g.n_kv));
     if (total > ((int64_t)1 << 30))
         return fail(BKV_ERR_INVALID, "append: more than 2^30 tokens in one call");
     return need_device(p);
@@ -2106,6 +2110,10 @@ static bkv_status read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
         most = std::max(most, n_cells[i]);
         if (total > ((int64_t)1 << 30)) return fail(BKV_ERR_INVALID, "read_rows: more than 2^30 cells in one call");
     }
+    // (a launch has fewer than 2^32 threads along an axis, one for each four values or 256 for each page and kv head)
+    if (((int64_t)most / p->g.page_cells + 2) * p->g.n_kv * std::max(4 * p->g.hd, 256) >= (int64_t)1 << 32)
+        return fail(BKV_ERR_INVALID, sfmt("read_rows: %lld cells of one sequence in a call are more than a launch takes at %lld kv heads", most,
+                                          p->g.n_kv));
     bkv_status st = need_device(p);
     if (st != BKV_OK) return st;
     if (total == 0) return flush_tables(p, S(stream));

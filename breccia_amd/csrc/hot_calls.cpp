@@ -34,7 +34,7 @@ PyObject* g_handle_name = nullptr;
 // The library's entry points; null until bind().
 #define ENTRY_POINTS(X) \
     X(bkv_append) X(bkv_append_f16) X(bkv_append_kprep) X(bkv_decode_attn) X(bkv_decode_step) X(bkv_decode_attn_select) \
-    X(bkv_prefill_attn) X(bkv_idx_pool) X(bkv_select_blocks) X(bkv_seq_reserve)
+    X(bkv_prefill_attn) X(bkv_idx_pool) X(bkv_select_blocks) X(bkv_seq_reserve) X(bkv_read_rows) X(bkv_read_rows_f16)
 #define POINTER(name) decltype(&::name) name = nullptr;
 struct Library {
     ENTRY_POINTS(POINTER)
@@ -177,6 +177,26 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                                          static_cast<const uint16_t*>(v), stream)
                         : g_lib.bkv_append(pool, layer, (int32_t)n, seqs, pos0, n_tokens, static_cast<const float*>(k),
                                      static_cast<const float*>(v), stream);
+    });
+}
+
+PyObject* read_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    Reader r(args, n_args, 9);
+    bkv_pool* pool = r.pool();
+    const int32_t layer = r.i32();
+    Py_ssize_t n, n1, n2;
+    const int32_t* seqs = r.i32s(n);
+    const int64_t* cell0 = r.i64s(n1);
+    const int32_t* n_cells = r.i32s(n2);
+    void *k = const_cast<void*>(r.device()), *v = const_cast<void*>(r.device());
+    void* stream = r.stream();
+    const bool f16_rows = r.flag();
+    if (!r.ok || n != n1 || n != n2 || n > INT32_MAX) return not_plain();
+    return status_of([&] {
+        return f16_rows ? g_lib.bkv_read_rows_f16(pool, layer, (int32_t)n, seqs, cell0, n_cells, static_cast<uint16_t*>(k),
+                                                  static_cast<uint16_t*>(v), stream)
+                        : g_lib.bkv_read_rows(pool, layer, (int32_t)n, seqs, cell0, n_cells, static_cast<float*>(k),
+                                              static_cast<float*>(v), stream);
     });
 }
 
@@ -396,6 +416,7 @@ PyMethodDef g_methods[] = {HOT_CALL(append),
                            HOT_CALL(idx_pool),
                            HOT_CALL(select_blocks),
                            HOT_CALL(seq_reserve),
+                           HOT_CALL(read_rows),
                            HOT_CALL(bind),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_hot", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -23,7 +23,7 @@ except ImportError as e:
     class _hot:  # noqa: N801
         """Takes no call."""
         append = append_kprep = decode_attn = decode_step = decode_attn_select = prefill_attn = idx_pool = select_blocks = \
-            seq_reserve = bind = staticmethod(lambda *args: NotImplemented)
+            seq_reserve = read_rows = bind = staticmethod(lambda *args: NotImplemented)
 
 
 _I32, _I64 = np.dtype(np.int32), np.dtype(np.int64)
@@ -529,6 +529,9 @@ class Pool:
     def read_rows(self, layer: int, seqs, cell0, n_cells, k_out_dev, v_out_dev, stream=None, f16_rows: bool = False) -> None:
         """Cells cell0[i] .. cell0[i] + n_cells[i] - 1 of sequence i as rows one after the other, f32 (or binary16 when f16_rows
         is set) [sum n_cells][n_kv_head][head_dim]: the way back from append."""
+        done = _hot.read_rows(self.handle, layer, seqs, cell0, n_cells, k_out_dev, v_out_dev, stream, f16_rows)
+        if done is not NotImplemented:
+            return check(done) if done else None
         seqs, ps = _i32(seqs)
         cell0, pc = _i64(cell0)
         n_cells, pn = _i32(n_cells)

@@ -165,7 +165,8 @@ _BENCH_SIGNATURES = {
 
 # entry points that kv.py also calls past ctypes (csrc/hot_calls.cpp)
 HOT_ENTRY_POINTS = ("bkv_append", "bkv_append_f16", "bkv_append_kprep", "bkv_decode_attn", "bkv_decode_step",
-                    "bkv_decode_attn_select", "bkv_prefill_attn", "bkv_idx_pool", "bkv_select_blocks", "bkv_seq_reserve")
+                    "bkv_decode_attn_select", "bkv_prefill_attn", "bkv_idx_pool", "bkv_select_blocks", "bkv_seq_reserve",
+                    "bkv_read_rows", "bkv_read_rows_f16")
 
 _bench_error = None   # message of the last failed call into the bench library, until check() takes it
 

@@ -99,3 +99,36 @@ def test_attention_of_such_a_pool_keeps_its_checks():
         expect(L.ERR_INVALID, p.decode_step, 0, [s, s], [5, 6], z, z, 16, z, z, 0.0625)
         expect(L.ERR_RANGE, p.decode_step, 0, [s], [40], z, z, 16, z, z, 0.0625)
         expect(L.ERR_NO_DEVICE, p.prefill_attn, 0, [s], [0], [40], 16, z, z, 0.0625)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_reading_back_takes_the_short_way(f16):
+    one = np.array([1], np.int32)
+    z = 0x1000
+    with Pool(layout=L.LAYOUT_F8P, n_pages=16, max_seqs=2, host_only=True) as p:
+        s = np.array([p.seq_create()], np.int32)
+        p.seq_reserve(int(s[0]), 17)
+        for cell, status in ((0, L.ERR_NO_DEVICE), (-1, L.ERR_RANGE)):
+            at = np.array([cell], np.int64)
+            assert kv._hot.read_rows(p.handle, 0, s, at, one, z, z, None, f16) == status
+            fast = expect(status, p.read_rows, 0, s, at, one, z, z, f16_rows=f16)
+            assert fast == expect(status, p.read_rows, 0, s.tolist(), at.tolist(), [1], z, z, f16_rows=f16)
+        assert kv._hot.read_rows(p.handle, 0, s, at, np.array([1, 1], np.int32), z, z, None, f16) is NotImplemented
+
+
+def test_what_no_launch_takes_is_refused():
+    # 256 threads for each page, kv head and side; 2^32 threads an axis
+    z = C.c_void_p(0x1000)
+    with Pool(layout=L.LAYOUT_F8P, n_pages=600_000, n_kv_head=16, max_seqs=2, max_pages_per_seq=600_000, host_only=True) as p:
+        s = p.seq_create()
+        most = 16 * ((1 << 32) // (16 * 512) - 2)
+        p.seq_reserve(s, most + 4096)
+        assert "more than a launch takes" in expect(L.ERR_INVALID, p.append, 0, [s], [5], [most], z, z)
+        assert "more than a launch takes" in expect(L.ERR_INVALID, p.append_kprep, 0, [s], [5], [most], z, z, z, 1e-6, z, 64, 16)
+        expect(L.ERR_NO_DEVICE, p.append, 0, [s], [5], [most - 1], z, z)
+    with Pool(layout=L.LAYOUT_F16, n_pages=600_000, n_kv_head=16, max_seqs=2, max_pages_per_seq=600_000, host_only=True) as p:
+        s = p.seq_create()
+        p.seq_reserve(s, 16 * 600_000)
+        most = 16 * ((1 << 32) // (16 * 1024) - 2)
+        assert "more than a launch takes" in expect(L.ERR_INVALID, p.read_rows, 0, [s], [5], [most], z, z)
+        expect(L.ERR_NO_DEVICE, p.read_rows, 0, [s], [5], [most - 1], z, z)
