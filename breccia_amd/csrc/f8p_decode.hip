@@ -129,8 +129,8 @@ struct Walk {
 // SEL: the cells of a list of 4-cell blocks instead of all; a wave's unit is then a group of four listed blocks, which stand for
 // the four blocks of a page.
 // ONCE: the pages go past the caches.  What a call of many pages leaves there is gone before anyone comes back to it, and its way
-// in costs: sixteen contexts of 8k to 128k 255 -> 225 us (5.5 -> 6.3 TB/s), eight of 1k to 32k 36.5 -> 32.3.  Eight of 10000,
-// which stay in the 256 MB behind the dies' caches between two calls, 21.4 -> 22.2.
+// in costs: sixteen contexts of 8k to 128k 250 -> 222 us (5.6 -> 6.3 TB/s), eight of 1k to 32k 33.4 -> 30.0.  Eight of 6000,
+// which stay in the 256 MB behind the dies' caches between two calls, 15.8 -> 18.0.
 template <bool SEL, bool ONCE, typename Args>
 __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P) {
     constexpr bool DESC = std::is_same<Args, AttnKernelParams>::value;
@@ -192,17 +192,21 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
         else return *(gptr_u4)at;
     };
     const auto block_at = [&](uint32_t id) { return (size_t)((min(id, (uint32_t)pos >> 2) & 3) * 1024); };
+    // (the exponents ahead of K: the scores wait for K alone, not for the V asked for since)
     const auto load_k = [&](int u) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             const int w = min(u + p, mine - 1) & (kAhead - 1);
             gptr at;
             if constexpr (SEL) {
+                ex[p] = *(gptr_i2)(gptr)(lines + (size_t)(unsigned)__shfl(ids, 4 * w + g, 64) * k_page);
                 const int from = 4 * w + (c >> 2);
                 const size_t page = (size_t)(unsigned)__shfl(ids, from, 64);
                 at = (gptr)(kpool + page * k_page + block_at((uint32_t)__shfl(blocks, from, 64))) + (g * 64 + (c & 3) * 16);
             } else {
-                at = (gptr)(kpool + (size_t)(unsigned)__builtin_amdgcn_readlane(ids, w) * k_page) + ((c >> 2) * 1024 + g * 64 + (c & 3) * 16);
+                const size_t page = (size_t)(unsigned)__builtin_amdgcn_readlane(ids, w);
+                ex[p] = *(gptr_i2)(gptr)(lines + page * k_page);
+                at = (gptr)(kpool + page * k_page) + ((c >> 2) * 1024 + g * 64 + (c & 3) * 16);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) k[p][i] = load(at + 256 * i);
@@ -212,20 +216,16 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             const int w = min(u + p, mine - 1) & (kAhead - 1);
-            size_t page;
             gptr at;
             if constexpr (SEL) {
                 const int from = 4 * w + g;
-                page = (size_t)(unsigned)__shfl(ids, from, 64);
                 vb[p] = __shfl(blocks, from, 64);
-                at = (gptr)(vpool + page * v_page + block_at((uint32_t)vb[p])) + c * 16;
+                at = (gptr)(vpool + (size_t)(unsigned)__shfl(ids, from, 64) * v_page + block_at((uint32_t)vb[p])) + c * 16;
             } else {
-                page = (size_t)(unsigned)__builtin_amdgcn_readlane(ids, w);
-                at = (gptr)(vpool + page * v_page) + (g * 1024 + c * 16);
+                at = (gptr)(vpool + (size_t)(unsigned)__builtin_amdgcn_readlane(ids, w) * v_page) + (g * 1024 + c * 16);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[p][i] = load(at + 256 * i);
-            ex[p] = *(gptr_i2)(gptr)(lines + page * k_page);
         }
     };
 
@@ -236,16 +236,21 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
     }
     if constexpr (!SEL) fetch_q();
     W.split_q(raw, P.scale_log2e);
-    for (int u = 0; u < mine; u += 2) {
-        const bool more = u + 2 < mine;
+    // Two forms of a step, the last one asks for nothing: of one with branches around its loads the compiler cannot tell what is in
+    // flight behind them, and waits for V with K (eight contexts of 1k to 32k 31.2 us instead of 30.0).
+    const auto step = [&](int u, auto asks) __attribute__((always_inline)) {
+        constexpr bool more = decltype(asks)::value;
         int ek[2], ev[2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) ek[p] = f8p_exponent_read(ex[p].x), ev[p] = f8p_exponent_read(ex[p].y);
         float z[2][4];
         unsigned live_v[2] = {0xffffffffu, 0xffffffffu};
         W.scores(k, ek, ev, z);
-        if (more) {
-            if (((u + 2) & (kAhead - 1)) == 0) fetch_ids(u + 2);
+        if constexpr (more) {
+            if (((u + 2) & (kAhead - 1)) == 0) {
+                fetch_ids(u + 2);
+                asm volatile("" : "+v"(ids));  // waited for here: behind the branch every trip would wait for the V it has in flight
+            }
             load_k(u + 2);
         }
         if constexpr (SEL) {
@@ -259,7 +264,7 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
                     live_v[p] |= live ? 0xffu << (8 * r) : 0u;
                 }
             }
-        } else if (!more) {
+        } else if constexpr (!more) {
             // cells past the position, and the page asked for twice
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
         }
         f8_h8 ph, pl;
         W.softmax(z, ev, ph, pl);
-        if (SEL || !more) {
+        if constexpr (SEL || !more) {
             // values that no weight belongs to may be anything (a weight of 0 would not keep NaN away)
 #pragma unroll
             for (int p = 0; p < 2; ++p)
@@ -279,8 +284,11 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
                 for (int i = 0; i < 4; ++i) v[p][i] &= live_v[p];
         }
         W.add_values(v, ph, pl);
-        if (more) load_v(u + 2);
-    }
+        if constexpr (more) load_v(u + 2);
+    };
+    int last = 0;
+    for (; last + 2 < mine; last += 2) step(last, std::true_type{});
+    if (mine > 0) step(last, std::false_type{});
 
     // ---- the four waves' results folded; wave w sums columns 64 w .. 64 w + 63 and writes them ----
     W.l = sum_over_lane_groups(W.l);
@@ -318,7 +326,7 @@ __global__ __launch_bounds__(kBlock, 2) void decode_attn_f8p_kernel(const Args P
 }
 
 // Bytes from which on pages go past the caches (ONCE): what the calls of one token walk, of all layers of the pool, before they come
-// back to the first page.  (Eight contexts of 12000, 94 MiB: 23.3 us kept, 23.7 past; of 14000, 109 MiB: 28.5 kept, 26.5 past.)
+// back to the first page.  (Eight contexts of 12000, 94 MiB: 22.3 us kept, 22.6 past; of 14000, 109 MiB: 26.3 kept, 25.2 past.)
 constexpr int64_t kOnceFrom = 96ll << 20;
 
 }  // namespace
