@@ -244,6 +244,8 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  * scale brings below 2^-6 * 2^e and which are rounded again, by at most 2^-10 * 2^e; cells behind the last one written are
  * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, and two entries of
  * one call must not write the same page (BKV_ERR_INVALID).  What a page holds depends on the rows written into it alone.
+ * bkv_decode_step, and a step plan's decode, are the write's launch and then the attention's.  A call writes fewer than 2^23 pages
+ * x kv heads of one sequence (BKV_ERR_INVALID otherwise).
  * A K page is n_kv_head units of 4096 bytes and a line of 128 with the exponents, int32 [kv head][K, V]; a V page n_kv_head units.
  * In a unit, value d of cell c is at byte
  *   K   1024 (c / 4) + 64 (8 (d / 128) + d / 4 % 8) + 16 (c % 4) + 4 (d / 32 % 4) + d % 4
@@ -348,8 +350,8 @@ bkv_status bkv_decode_attn_static(bkv_pool *pool, int32_t layer, int32_t n, cons
  * as the exact f16 the cache holds; q and the probabilities are f32 split into two f16 parts,
  * so accuracy is that of f32 accumulation.  q8_0 V blocks (BRECCIA_KV_Q8V in
  * qsa_attn_apply_gqa.comp:53-77) are dequantised once per work-group into two f16 terms whose
- * sum carries code * scale to 22 bits, and so are int8 K blocks.  All three layouts, head_dim
- * 256, 16-cell pages.  Written
+ * sum carries code * scale to 22 bits, and so are int8 K blocks; e4m3 codes are f16 numbers, their
+ * scales join the scores and the weights.  All layouts, head_dim 256, 16-cell pages.  Written
  * for chunks of tens to thousands of tokens; a handful of tokens is bkv_decode_attn's case.
  * A call whose longest page walks would outlast the rest of it (few rows, or very unequal
  * contexts on the quantised layouts) has them cut into ranges: two kernels, with partial results
@@ -414,7 +416,7 @@ bkv_status bkv_decode_step(bkv_pool *pool, int32_t layer, int32_t n, const int32
  * an event recorded there at that moment, and behind the last block-table scatter wherever that
  * ran.  A replayed graph holds none of these host-made orderings: replay on the stream the capture
  * was taken from, or order the streams yourself.  Destroy a pool's plans before the pool
- * (bkv_pool_destroy returns BKV_ERR_STATE while one is alive).  All three layouts. */
+ * (bkv_pool_destroy returns BKV_ERR_STATE while one is alive).  All layouts. */
 typedef struct bkv_step_plan bkv_step_plan;
 bkv_status bkv_step_plan_create(bkv_pool *pool, int32_t n, const int32_t *seqs, const int64_t *pos,
                                 int32_t horizon, int32_t n_q_head, void *stream, bkv_step_plan **out);
