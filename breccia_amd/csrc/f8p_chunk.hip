@@ -9,8 +9,9 @@
 // What bounds it: power first (1.85 to 2.1 GHz under it), then issue.  q and the weights are two f16 numbers each, so twice the
 // useful products are issued; a library product reaches 1245 TFLOP/s on this card, and four chunks of 1024 tokens behind 1536 take
 // 221 us, as long as their products would there.  A prompt of 4096 at 12 heads a kv head takes 370 of 331: the start and the end
-// of its 768 work-groups are a tenth of their time (an order of dispatch that evens out when they end brought 1 %).  16x16x32 products and two tiles because 32x32x16 ones cost more power (from registers alone
-// 1403 TFLOP/s against 1647); pages shared through LDS took 250 us where this took 242.
+// of its 768 work-groups are a tenth of their time (an order of dispatch that evens out when they end brought 1 %).  16x16x32
+// products and two tiles because 32x32x16 ones cost more power (from registers alone 1403 TFLOP/s against 1647); pages shared
+// through LDS took 250 us where this took 242.
 #include <type_traits>
 
 #include "f8p_attn.hpp"

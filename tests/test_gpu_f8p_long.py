@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 
 import f8p_model as M
+import oracle
 from breccia_amd import lib as L
-from breccia_amd.kv import DeviceBuffer, Pool, Stream, device_sync, rope_table
+from breccia_amd.kv import DeviceBuffer, Graph, Pool, Stream, device_sync, rope_table
 from gpu_common import REF_BAR_MAX_REL, check_attn
 from test_gpu_f8p import cells_at, chunk, fill, lists, rng_of, rows_of
 
@@ -194,3 +195,51 @@ def test_two_pools_on_two_streams():
             assert np.array_equal(od.download(np.float32).reshape(w[1].shape), w[1])
             for got, rows in zip((ko, vo), cells_at(tw, 0, s, 1500)):
                 assert np.array_equal(got.download(np.uint16).view(np.float16).reshape(rows.shape), rows.astype(np.float16))
+
+
+def test_captured_writes_reads_and_attention_replay():
+    # the same cells written again by every replay from buffers that change, eager calls of another sequence in between
+    rng = rng_of(39)
+    n_q, n = 16, 45
+    gamma, table = np.ones(256, np.float32), rope_table(1e6, 64, 128)
+    with M.F8Twin(n_pages=32) as tw:
+        pool, st = tw.pool, Stream()
+        a, other = pool.seq_create(), pool.seq_create()
+        for s in (a, other):
+            pool.seq_reserve(s, 100)
+            fill(tw, s, 60, rng)
+        kd, vd, hk, hv, qd = (DeviceBuffer(x) for x in (n * 2 * 1024, n * 2 * 1024, 7 * 2 * 512, 7 * 2 * 512, n_q * 1024))
+        gd, td = DeviceBuffer.from_numpy(gamma), DeviceBuffer.from_numpy(table)
+        od, ko, vo = DeviceBuffer(n_q * 1024), DeviceBuffer(100 * 2 * 1024), DeviceBuffer(100 * 2 * 1024)
+
+        def calls(stream):
+            pool.append(0, [a], [41], [7], hk, hv, stream=stream, f16_rows=True)
+            pool.append_kprep(0, [a], [48], [n], kd, vd, gd, 1e-6, td, 64, 128, stream=stream)
+            pool.decode_attn_static(0, [a], [92], n_q, qd, od, 1 / 16.0, stream=stream)
+            pool.read_rows(0, [a], [0], [93], ko, vo, stream=stream)
+
+        st.sync()
+        graph = Graph(st)
+        calls(st)
+        graph.end()
+        for turn in range(4):
+            k, v, q = rows_of(rng, n, 2, 1.0 + turn), rows_of(rng, n, 2, 2.0 ** turn), rng.standard_normal((1, n_q, 256)).astype(np.float32)
+            h = [rows_of(rng, 7, 2, 2.0 ** -turn).astype(np.float16) for _ in range(2)]
+            for buf, x in ((kd, k), (vd, v), (qd, q), (hk, h[0].view(np.uint16)), (hv, h[1].view(np.uint16))):
+                buf.upload(x, st)
+            graph.launch()
+            got = [b.download(np.float32, count, st) for b, count in ((od, n_q * 256), (ko, 93 * 512), (vo, 93 * 512))]
+            x = rows_of(rng, 10, 2)
+            tw.append(0, [other], [60], [x], [x])
+            # the cache's load rule: codes of exponent field 0 read as signed zeros
+            wide = [np.where(np.abs(x) < 2.0 ** -14, np.copysign(np.float32(0), x), x).astype(np.float32) for x in h]
+            tw.images[0].append(pool.block_table(a), 41, *wide)
+            tok = (48 + np.arange(n)).astype(np.int32)
+            tw.images[0].append(pool.block_table(a), 48, oracle.k_prep(k, 2, 256, gamma, 1e-6, table, 64, tok), v)
+            tw.assert_pools_equal()
+            ck, cv = cells_at(tw, 0, a, 93)
+            assert np.array_equal(got[1].reshape(ck.shape), ck) and np.array_equal(got[2].reshape(cv.shape), cv)
+            assert check_attn(got[0].reshape(n_q, 256), M.attend64(q, ck, cv, [range(93)], 1 / 16.0)[0])[1] <= REF_BAR_MAX_REL
+            calls(st)
+            assert np.array_equal(od.download(np.float32, n_q * 256, st), got[0])
+        graph.destroy()
