@@ -872,9 +872,8 @@ static bkv_status build_append_batch(bkv_pool* p, int32_t layer, int32_t n_seqs,
     }
     b.n = n_seqs;
     // (a launch has fewer than 2^32 threads along an axis, 256 of them for each page, kv head and side)
-    if (p->g.layout == BKV_LAYOUT_F8P && ((int64_t)max_tok / p->g.page_cells + 2) * p->g.n_kv * 512 >= (int64_t)1 << 32)
-        return fail(BKV_ERR_INVALID, sfmt("append: %lld rows of one sequence in a call are more than a launch takes at %lld kv heads", max_tok,
-                                          p->g.n_kv));
+    if (p->g.layout == BKV_LAYOUT_F8P && (total / p->g.page_cells + 2 * n_seqs) * p->g.n_kv * 512 >= (int64_t)1 << 32)
+        return fail(BKV_ERR_INVALID, sfmt("append: %lld rows in a call are more than a launch takes at %lld kv heads", total, p->g.n_kv));
     if (total > ((int64_t)1 << 30))
         return fail(BKV_ERR_INVALID, "append: more than 2^30 tokens in one call");
     return need_device(p);
@@ -2071,7 +2070,7 @@ bkv_status bkv_gather(bkv_pool* p, int32_t layer, int32_t seq, int64_t cell0, in
         AppendBatch b{};
         b.n = 1;
         b.row[0] = seq, b.pos0[0] = (int32_t)cell0, b.n_tok[0] = (int32_t)n;
-        BKV_HIP(launch_read_rows(p, layer, b, (int32_t)n, k_out_dev, v_out_dev, false, S(stream)));
+        BKV_HIP(launch_read_rows(p, layer, b, n, k_out_dev, v_out_dev, false, S(stream)));
         return BKV_OK;
     }
     BKV_HIP(launch_gather(p, layer, seq, cell0, n, k_out_dev, v_out_dev, S(stream)));
@@ -2090,7 +2089,6 @@ static bkv_status read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
     AppendBatch b{};
     b.n = n_seqs;
     int64_t total = 0;
-    int32_t most = 0;
     for (int i = 0; i < n_seqs; ++i) {
         if (!p->alloc->seq_valid(seqs[i])) return fail(BKV_ERR_RANGE, sfmt("read_rows: sequence %lld is not live", seqs[i]));
         if (n_cells[i] < 0 || cell0[i] < 0 || cell0[i] > p->alloc->seq_capacity(seqs[i]) - n_cells[i])
@@ -2107,13 +2105,11 @@ static bkv_status read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
         b.n_tok[i] = n_cells[i];
         b.src0[i] = (int32_t)total;
         total += n_cells[i];
-        most = std::max(most, n_cells[i]);
         if (total > ((int64_t)1 << 30)) return fail(BKV_ERR_INVALID, "read_rows: more than 2^30 cells in one call");
     }
     // (a launch has fewer than 2^32 threads along an axis, one for each four values or 256 for each page and kv head)
-    if (((int64_t)most / p->g.page_cells + 2) * p->g.n_kv * std::max(4 * p->g.hd, 256) >= (int64_t)1 << 32)
-        return fail(BKV_ERR_INVALID, sfmt("read_rows: %lld cells of one sequence in a call are more than a launch takes at %lld kv heads", most,
-                                          p->g.n_kv));
+    if ((total / p->g.page_cells + 2 * n_seqs) * p->g.n_kv * std::max(4 * p->g.hd, 256) >= (int64_t)1 << 32)
+        return fail(BKV_ERR_INVALID, sfmt("read_rows: %lld cells in a call are more than a launch takes at %lld kv heads", total, p->g.n_kv));
     bkv_status st = need_device(p);
     if (st != BKV_OK) return st;
     if (total == 0) return flush_tables(p, S(stream));
@@ -2121,7 +2117,7 @@ static bkv_status read_rows(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
         return fail(BKV_ERR_INVALID, "read_rows: output device pointers must be non-NULL and 16-byte aligned");
     st = flush_tables(p, S(stream));
     if (st != BKV_OK) return st;
-    BKV_HIP(launch_read_rows(p, layer, b, most, k_out_dev, v_out_dev, to_f16, S(stream)));
+    BKV_HIP(launch_read_rows(p, layer, b, total, k_out_dev, v_out_dev, to_f16, S(stream)));
     return BKV_OK;
 }
 

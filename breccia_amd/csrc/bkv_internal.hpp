@@ -207,7 +207,7 @@ hipError_t launch_append_kprep(bkv_pool* p, int32_t layer, const AppendBatch& b,
                                const float* table, int32_t n_rot, int32_t max_pos,
                                const int32_t* positions, hipStream_t stream);
 
-// The e4m3 layout (f8p_move.hip): a work-group per (page, kv head) written.  _desc: one token of every entry of a step plan's
+// The e4m3 layout (f8p_move.hip): work-groups for each (page, kv head) written.  _desc: one token of every entry of a step plan's
 // descriptor, at its position.
 hipError_t launch_append_f8p(bkv_pool* p, int32_t layer, const AppendBatch& b, const void* k, const void* v, bool src_is_f16,
                              hipStream_t stream);
@@ -217,7 +217,7 @@ hipError_t launch_append_kprep_f8p(bkv_pool* p, int32_t layer, const AppendBatch
 hipError_t launch_append_f8p_desc(bkv_pool* p, int32_t layer, const AttnBatch* desc, int32_t n, const float* k, const float* v,
                                   hipStream_t stream);
 // Cells pos0[i] .. pos0[i] + n_tok[i] - 1 as rows from src0[i] on, f32 or binary16; every layout.
-hipError_t launch_read_rows(bkv_pool* p, int32_t layer, const AppendBatch& b, int32_t max_cells, void* k, void* v, bool to_f16,
+hipError_t launch_read_rows(bkv_pool* p, int32_t layer, const AppendBatch& b, int64_t rows, void* k, void* v, bool to_f16,
                             hipStream_t stream);
 
 // Block selection (select.hip): one entry per (token) list.

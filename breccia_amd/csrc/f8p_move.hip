@@ -127,33 +127,56 @@ __device__ __forceinline__ F8Old old_of(const F8Target& t, const F8Share& at) {
     return F8Old{*reinterpret_cast<const v4u*>(V ? t.vunit + at.v_at : t.kunit + at.k_at), f8p_exponent_read(t.line[V])};
 }
 
-// Which of a launch's work a work-group has: (page of the entry, kv head, K or V), both halves of a (page, kv head) side by side,
-// in turns so that the dies, which have every eighth work-group, get as much of K as of V.
+// Which entry's page a work-group has.  By the grid: a row of it for each entry, as long as the longest (AppendBatchOf); or, where
+// that leaves many work-groups with nothing, by a search of the entries, the grid as long as the batch has pages (F8Batch).
+// find: `at`, which page of the launch, becomes which page of the entry; false where there is none.
+struct F8Rows {
+    int row, pos0, n_tok, src0;
+};
+__host__ __device__ inline int pages_touched(int pos0, int n_tok) { return n_tok > 0 ? (pos0 + (n_tok - 1)) / kF8Page - pos0 / kF8Page + 1 : 0; }
+template <int N>
+__device__ __forceinline__ bool find(const AppendBatchOf<N>& b, int& at, F8Rows& r) {
+    const int e = blockIdx.y;
+    r = F8Rows{b.row[e], b.pos0[e], b.n_tok[e], b.src0[e]};
+    return at < pages_touched(r.pos0, r.n_tok);
+}
+// base[i]: pages of the entries before i; behind the last one INT32_MAX
+template <int N>
+struct F8Batch : AppendBatchOf<N> {
+    int32_t base[N];
+};
+template <int N>
+__device__ __forceinline__ bool find(const F8Batch<N>& b, int& at, F8Rows& r) {
+    int e = -1;
+#pragma unroll
+    for (int i = 0; i < N; ++i) e += at >= b.base[i] ? 1 : 0;
+    at -= b.base[e];
+    r = F8Rows{b.row[e], b.pos0[e], b.n_tok[e], b.src0[e]};
+    return true;
+}
+// a step plan's: one token of every entry of the descriptor
+struct F8DescBatch {
+    const AttnBatch* bd;
+};
+__device__ __forceinline__ bool find(const F8DescBatch& b, int& at, F8Rows& r) {
+    const int e = blockIdx.y;
+    r = F8Rows{b.bd->row[e], b.bd->pos[e], 1, e};
+    return true;
+}
+
+// Which of a launch's work a work-group has, of which there is one for (page, kv head, K or V): both halves of a (page, kv head)
+// side by side, in turns so that the dies, which have every eighth work-group, get as much of K as of V.
 struct F8Work {
-    int at_page, kvh;
+    int page, kvh;  // page: of the launch
     bool v;
 };
 __device__ __forceinline__ F8Work work_of(int x, int n_kv) {
     F8Work w;
     w.v = ((x ^ (x >> 3)) & 1) != 0;
-    w.at_page = (x >> 1) / n_kv;
-    w.kvh = (x >> 1) - w.at_page * n_kv;
+    w.page = (x >> 1) / n_kv;
+    w.kvh = (x >> 1) - w.page * n_kv;
     return w;
 }
-
-// One work-group per (page of an entry, kv head): grid (pages of the longest entry x kv heads, entries).
-// Batch: of the call, or (a step plan's) one token of every entry of the descriptor.
-struct F8Rows {
-    int row, pos0, n_tok, src0;
-};
-template <typename Batch>
-__device__ __forceinline__ F8Rows rows_of(const Batch& b, int s) {
-    return F8Rows{b.row[s], b.pos0[s], b.n_tok[s], b.src0[s]};
-}
-struct F8DescBatch {
-    const AttnBatch* bd;
-};
-__device__ __forceinline__ F8Rows rows_of(const F8DescBatch& b, int s) { return F8Rows{b.bd->row[s], b.bd->pos[s], 1, s}; }
 
 // The rows of a work-group's page: where they come from, which of them the call writes.
 struct F8Span {
@@ -192,10 +215,10 @@ __global__ __launch_bounds__(kBlock) void append_f8p_kernel(Batch b, F8MoveGeom 
                                                             const int32_t* __restrict__ tables, const SrcT* __restrict__ ks,
                                                             const SrcT* __restrict__ vs) {
     __shared__ float red[kF8Waves];
-    const F8Rows r = rows_of(b, blockIdx.y);
-    const F8Work w = work_of(blockIdx.x, g.n_kv);
-    const F8Span s = span_of(r, w.at_page);
-    if (s.end <= 0 || r.n_tok == 0) return;
+    F8Work w = work_of(blockIdx.x, g.n_kv);
+    F8Rows r;
+    if (!find(b, w.page, r)) return;
+    const F8Span s = span_of(r, w.page);
     const F8Target t = target_of(g, kpool, vpool, tables, r.row, s.page, w.kvh);
     if (w.v) append_unit<true>(r, s, g.n_kv, w.kvh, t, vs, red);
     else append_unit<false>(r, s, g.n_kv, w.kvh, t, ks, red);
@@ -214,17 +237,19 @@ struct F8Prep {
     int32_t n_rot, max_pos;
 };
 constexpr int kPrepStride = kF8Hd + 4;
-__global__ __launch_bounds__(kBlock, 8) void append_kprep_f8p_kernel(AppendBatch b, F8MoveGeom g, F8Prep kp, uint8_t* __restrict__ kpool,
+template <typename Batch>
+__global__ __launch_bounds__(kBlock, 8) void append_kprep_f8p_kernel(Batch b, F8MoveGeom g, F8Prep kp, uint8_t* __restrict__ kpool,
                                                                      uint8_t* __restrict__ vpool, const int32_t* __restrict__ tables,
                                                                      const float* __restrict__ ks, const float* __restrict__ vs) {
 #pragma clang fp contract(off)
     __shared__ float red_v[kF8Waves], red_k[kF8Waves];
     __shared__ __attribute__((aligned(16))) float rows_s[kF8Page * kPrepStride];
     __shared__ double inv_s[kF8Page];
-    const F8Rows r = rows_of(b, blockIdx.y);
-    const int at_page = (int)blockIdx.x / g.n_kv, kvh = (int)blockIdx.x - at_page * g.n_kv;
+    int at_page = (int)blockIdx.x / g.n_kv;
+    const int kvh = (int)blockIdx.x - at_page * g.n_kv;
+    F8Rows r;
+    if (!find(b, at_page, r)) return;
     const F8Span s = span_of(r, at_page);
-    if (s.end <= 0 || r.n_tok == 0) return;
     const int tid = threadIdx.x;
     const F8Share at(tid);
     const F8Target t = target_of(g, kpool, vpool, tables, r.row, s.page, kvh);
@@ -292,7 +317,7 @@ __global__ __launch_bounds__(kBlock, 8) void append_kprep_f8p_kernel(AppendBatch
 
 // ---- rows read back -----------------------------------------------------------------------------------
 // The values of cells cell0[i] .. of sequence i as rows [sum n_tok][n_kv][hd], f32 or binary16 (rounded to nearest).
-// AppendBatch: pos0 = first cell, n_tok = cells, src0 = first row of the output.
+// The batch's pos0 = first cell, n_tok = cells, src0 = first row of the output.
 __device__ __forceinline__ void put4(float* p, const float (&x)[4]) {
     __builtin_nontemporal_store(v4u{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])}, reinterpret_cast<v4u*>(p));
 }
@@ -317,11 +342,11 @@ template <typename DstT, typename Batch>
 __global__ __launch_bounds__(kBlock) void read_rows_f8p_kernel(Batch b, F8MoveGeom g, const uint8_t* __restrict__ kpool,
                                                                const uint8_t* __restrict__ vpool, const int32_t* __restrict__ tables,
                                                                DstT* __restrict__ ko, DstT* __restrict__ vo) {
-    const F8Rows r = rows_of(b, blockIdx.y);
-    const int first_page = r.pos0 / kF8Page;
-    const int at_page = (int)blockIdx.x / g.n_kv, kvh = (int)blockIdx.x - at_page * g.n_kv;
-    const int page = first_page + at_page;
-    if (r.n_tok == 0 || page > (r.pos0 + r.n_tok - 1) / kF8Page) return;
+    int at_page = (int)blockIdx.x / g.n_kv;
+    const int kvh = (int)blockIdx.x - at_page * g.n_kv;
+    F8Rows r;
+    if (!find(b, at_page, r)) return;
+    const int page = r.pos0 / kF8Page + at_page;
     const F8Share at(threadIdx.x);
     const F8Target t = target_of(g, const_cast<uint8_t*>(kpool), const_cast<uint8_t*>(vpool), tables, r.row, page, kvh);
     const F8Old k = old_of<false>(t, at), v = old_of<true>(t, at);
@@ -373,15 +398,20 @@ __global__ __launch_bounds__(kBlock) void read_rows_f8p_kernel(Batch b, F8MoveGe
 template <int LAYOUT, typename DstT, typename Batch>
 __global__ __launch_bounds__(kBlock) void read_rows_kernel(Batch b, F8MoveGeom g, int hd, const uint8_t* __restrict__ kpool,
                                                            const uint8_t* __restrict__ vpool, const int32_t* __restrict__ tables,
-                                                           DstT* __restrict__ ko, DstT* __restrict__ vo) {
-    const F8Rows r = rows_of(b, blockIdx.y);
+                                                           DstT* __restrict__ ko, DstT* __restrict__ vo, unsigned rows) {
     const unsigned per_cell = (unsigned)(g.n_kv * (hd / 4));
-    const int64_t idx = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (idx >= (int64_t)r.n_tok * per_cell) return;
-    const unsigned i = (unsigned)(idx / per_cell), rest = (unsigned)(idx - (int64_t)i * per_cell);
+    const unsigned idx = blockIdx.x * (unsigned)kBlock + threadIdx.x;  // (below 2^32: checked on the host)
+    const unsigned i = idx / per_cell, rest = idx - i * per_cell;
+    if (i >= rows) return;
     const unsigned kvh = rest / (unsigned)(hd / 4), d = 4 * (rest - kvh * (unsigned)(hd / 4));
-    const unsigned cell = (unsigned)r.pos0 + i;
-    const int32_t phys = tables[(size_t)r.row * (size_t)g.max_pages_per_seq + cell / kF8Page];
+    // the entry of the work-group's first row, and from there on
+    int e = -1;
+#pragma unroll
+    for (int k = 0; k < (int)(sizeof(b.src0) / sizeof(b.src0[0])); ++k)
+        e += k < b.n && blockIdx.x * (unsigned)kBlock / per_cell >= (unsigned)b.src0[k] ? 1 : 0;
+    while (e + 1 < b.n && i >= (unsigned)b.src0[e + 1]) ++e;
+    const unsigned cell = (unsigned)b.pos0[e] + i - (unsigned)b.src0[e];
+    const int32_t phys = tables[(size_t)b.row[e] * (size_t)g.max_pages_per_seq + cell / kF8Page];
     const size_t row = ((size_t)phys * g.n_kv + kvh) * kF8Page + cell % kF8Page;
     const auto halves = [&](const uint8_t* pool, float (&x)[4]) {
         const v2u w = *reinterpret_cast<const v2u*>(pool + (row * (size_t)hd + d) * 2);
@@ -408,42 +438,61 @@ __global__ __launch_bounds__(kBlock) void read_rows_kernel(Batch b, F8MoveGeom g
             codes(w[1 + (d % 32) / 4], __uint_as_float(w[0]), v);
         }
     }
-    const size_t to = (((size_t)r.src0 + i) * (size_t)g.n_kv + kvh) * (size_t)hd + d;
+    const size_t to = ((size_t)i * (size_t)g.n_kv + kvh) * (size_t)hd + d;
     put4(ko + to, k);
     put4(vo + to, v);
 }
 
 F8MoveGeom f8_geom(const bkv_pool* p) { return F8MoveGeom{p->g.n_kv, p->desc.max_pages_per_seq}; }
 
-// pages the longest of the batch's entries touches
-unsigned pages_of(const AppendBatch& b) {
-    int most = 0;
-    for (int i = 0; i < b.n; ++i)
-        if (b.n_tok[i] > 0) most = std::max(most, (b.pos0[i] + b.n_tok[i] - 1) / kF8Page - b.pos0[i] / kF8Page + 1);
-    return (unsigned)most;
-}
-
-// f of the batch, in the smaller argument struct where it fits (kFewEntries)
-template <typename F>
-void with_batch(const AppendBatch& b, F f) {
-    if (b.n > kFewEntries) return f(b);
-    AppendBatchOf<kFewEntries> few{};
-    few.n = b.n;
+// f of the batch in the argument struct that suits it, and of the launch's grid, `each` work-groups a page: the smaller structs
+// where they fit (kFewEntries), a search of the entries where the other way leaves more than kIdle work-groups with nothing.
+// Those cost what starting them costs, the search a trip to the arguments, 0.7 us: one prompt of 8192 and 63 tokens beside it, 128k
+// of them idle, 71 us by the grid and 21 by the search; 64 chunks of 64, none, 12.0 and 13.6; five ragged chunks, 1552, 12.6 and 12.8.
+constexpr int64_t kIdle = 2048;
+template <typename Batch>
+void fill_batch(Batch& out, const AppendBatch& b) {
+    out.n = b.n;
     for (int i = 0; i < b.n; ++i) {
-        few.row[i] = b.row[i];
-        few.pos0[i] = b.pos0[i];
-        few.n_tok[i] = b.n_tok[i];
-        few.src0[i] = b.src0[i];
+        out.row[i] = b.row[i];
+        out.pos0[i] = b.pos0[i];
+        out.n_tok[i] = b.n_tok[i];
+        out.src0[i] = b.src0[i];
     }
-    f(few);
+}
+template <int N, typename F>
+void with_entries(const AppendBatch& b, int each, F f) {
+    int64_t pages = 0, most = 0;
+    for (int i = 0; i < b.n; ++i) {
+        const int n = pages_touched(b.pos0[i], b.n_tok[i]);
+        pages += n;
+        most = std::max<int64_t>(most, n);
+    }
+    if ((most * b.n - pages) * each <= kIdle) {
+        AppendBatchOf<N> out{};
+        fill_batch(out, b);
+        return f(out, dim3((unsigned)(most * each), (unsigned)b.n));
+    }
+    F8Batch<N> out{};
+    fill_batch(out, b);
+    int32_t base = 0;
+    for (int i = 0; i < N; ++i) {
+        out.base[i] = i < b.n ? base : INT32_MAX;
+        if (i < b.n) base += pages_touched(b.pos0[i], b.n_tok[i]);
+    }
+    f(out, dim3((unsigned)(pages * each)));
+}
+template <typename F>
+void with_batch(const AppendBatch& b, int each, F f) {
+    if (b.n > kFewEntries) with_entries<BKV_MAX_BATCH>(b, each, f);
+    else with_entries<kFewEntries>(b, each, f);
 }
 
 }  // namespace
 
 hipError_t launch_append_f8p(bkv_pool* p, int32_t layer, const AppendBatch& b, const void* k, const void* v, bool src_is_f16,
                              hipStream_t stream) {
-    const dim3 grid(pages_of(b) * (unsigned)p->g.n_kv * 2, (unsigned)b.n);
-    with_batch(b, [&](const auto& batch) {
+    with_batch(b, 2 * p->g.n_kv, [&](const auto& batch, dim3 grid) {
         using Batch = std::decay_t<decltype(batch)>;
         const auto launch = [&](auto kernel, auto ks, auto vs) {
             launch_staged(p, BKV_STAGE_APPEND, kernel, grid, dim3(kBlock), 0, stream, batch, f8_geom(p), p->k_layer[(size_t)layer],
@@ -465,39 +514,45 @@ hipError_t launch_append_f8p_desc(bkv_pool* p, int32_t layer, const AttnBatch* d
 hipError_t launch_append_kprep_f8p(bkv_pool* p, int32_t layer, const AppendBatch& b, const float* k, const float* v, const float* gamma,
                                    float eps, const float* table, int32_t n_rot, int32_t max_pos, const int32_t* positions,
                                    hipStream_t stream) {
-    const dim3 grid(pages_of(b) * (unsigned)p->g.n_kv, (unsigned)b.n);
-    launch_staged(p, BKV_STAGE_APPEND_KPREP, append_kprep_f8p_kernel, grid, dim3(kBlock), 0, stream, b, f8_geom(p),
-                  F8Prep{gamma, table, positions, eps, n_rot, max_pos}, p->k_layer[(size_t)layer], p->v_layer[(size_t)layer],
-                  (const int32_t*)p->table_dev, k, v);
+    with_batch(b, p->g.n_kv, [&](const auto& batch, dim3 grid) {
+        launch_staged(p, BKV_STAGE_APPEND_KPREP, append_kprep_f8p_kernel<std::decay_t<decltype(batch)>>, grid, dim3(kBlock), 0, stream, batch,
+                      f8_geom(p), F8Prep{gamma, table, positions, eps, n_rot, max_pos}, p->k_layer[(size_t)layer], p->v_layer[(size_t)layer],
+                      (const int32_t*)p->table_dev, k, v);
+    });
     return hipGetLastError();
 }
 
-hipError_t launch_read_rows(bkv_pool* p, int32_t layer, const AppendBatch& b, int32_t max_cells, void* k, void* v, bool to_f16,
+hipError_t launch_read_rows(bkv_pool* p, int32_t layer, const AppendBatch& b, int64_t rows, void* k, void* v, bool to_f16,
                             hipStream_t stream) {
     const uint8_t* const kpool = p->k_layer[(size_t)layer];
     const uint8_t* const vpool = p->v_layer[(size_t)layer];
     const int32_t* const tables = p->table_dev;
-    with_batch(b, [&](const auto& batch) {
-        using Batch = std::decay_t<decltype(batch)>;
-        const auto to = [&](auto* ko, auto* vo) {
-            using DstT = std::remove_pointer_t<decltype(ko)>;
-            if (p->g.layout == BKV_LAYOUT_F8P) {
-                launch_staged(p, BKV_STAGE_READ_ROWS, read_rows_f8p_kernel<DstT, Batch>, dim3(pages_of(b) * (unsigned)p->g.n_kv, (unsigned)b.n),
-                              dim3(kBlock), 0, stream, batch, f8_geom(p), kpool, vpool, tables, ko, vo);
-                return;
-            }
-            const int64_t threads = (int64_t)max_cells * p->g.n_kv * (p->g.hd / 4);
-            const dim3 grid((unsigned)((threads + kBlock - 1) / kBlock), (unsigned)b.n);
+    const auto with_outputs = [&](auto ko, auto vo) {
+        using DstT = std::remove_pointer_t<decltype(ko)>;
+        if (p->g.layout == BKV_LAYOUT_F8P)
+            return with_batch(b, p->g.n_kv, [&](const auto& batch, dim3 grid) {
+                launch_staged(p, BKV_STAGE_READ_ROWS, read_rows_f8p_kernel<DstT, std::decay_t<decltype(batch)>>, grid, dim3(kBlock), 0, stream, batch,
+                              f8_geom(p), kpool, vpool, tables, ko, vo);
+            });
+        const int64_t threads = rows * p->g.n_kv * (p->g.hd / 4);
+        const dim3 grid((unsigned)((threads + kBlock - 1) / kBlock));
+        const auto by_layout = [&](const auto& batch) {
+            using Batch = std::decay_t<decltype(batch)>;
             const auto launch = [&](auto kernel) {
-                launch_staged(p, BKV_STAGE_READ_ROWS, kernel, grid, dim3(kBlock), 0, stream, batch, f8_geom(p), p->g.hd, kpool, vpool, tables, ko, vo);
+                launch_staged(p, BKV_STAGE_READ_ROWS, kernel, grid, dim3(kBlock), 0, stream, batch, f8_geom(p), p->g.hd, kpool, vpool, tables, ko, vo,
+                              (unsigned)rows);
             };
             if (p->g.layout == BKV_LAYOUT_F16) launch(read_rows_kernel<BKV_LAYOUT_F16, DstT, Batch>);
             else if (p->g.layout == BKV_LAYOUT_Q8V) launch(read_rows_kernel<BKV_LAYOUT_Q8V, DstT, Batch>);
             else launch(read_rows_kernel<BKV_LAYOUT_I8H, DstT, Batch>);
         };
-        if (to_f16) to((uint16_t*)k, (uint16_t*)v);
-        else to((float*)k, (float*)v);
-    });
+        if (b.n > kFewEntries) return by_layout(b);
+        AppendBatchOf<kFewEntries> few{};
+        fill_batch(few, b);
+        by_layout(few);
+    };
+    if (to_f16) with_outputs((uint16_t*)k, (uint16_t*)v);
+    else with_outputs((float*)k, (float*)v);
     return hipGetLastError();
 }
 

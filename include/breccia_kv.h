@@ -245,7 +245,7 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, and two entries of
  * one call must not write the same page (BKV_ERR_INVALID).  What a page holds depends on the rows written into it alone.
  * bkv_decode_step, and a step plan's decode, are the write's launch and then the attention's.  A call writes fewer than 2^23 pages
- * x kv heads of one sequence (BKV_ERR_INVALID otherwise).
+ * x kv heads (BKV_ERR_INVALID otherwise).
  * A K page is n_kv_head units of 4096 bytes and a line of 128 with the exponents, int32 [kv head][K, V]; a V page n_kv_head units.
  * In a unit, value d of cell c is at byte
  *   K   1024 (c / 4) + 64 (8 (d / 128) + d / 4 % 8) + 16 (c % 4) + 4 (d / 32 % 4) + d % 4

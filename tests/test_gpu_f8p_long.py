@@ -243,3 +243,63 @@ def test_captured_writes_reads_and_attention_replay():
             calls(st)
             assert np.array_equal(od.download(np.float32, n_q * 256, st), got[0])
         graph.destroy()
+
+
+@pytest.mark.parametrize("n, longest", [(9, 700), (9, 3001), (40, 700)])    # few entries and many, by the grid and by the search
+def test_a_prompt_beside_single_tokens_and_empty_entries(n, longest):
+    # entries of very different lengths, none at all among them, first, last and in the middle
+    rng = rng_of(40, n)
+    lens = [0, 1, 0, 0, longest, 1, 1, 0, 33] + [int(x) for x in rng.integers(0, 2, max(n - 11, 0))] + [19, 0][:max(n - 9, 0)]
+    at = [int(x) for x in rng.integers(0, 40, n)]
+    gamma, table = (1 + 0.1 * rng.standard_normal(256)).astype(np.float32), rope_table(1e7, 64, 8192)
+    with M.F8Twin(n_pages=500, max_seqs=n) as tw:
+        pool = tw.pool
+        pool.set_free_order(rng.permutation(500).astype(np.int32))
+        seqs = [pool.seq_create() for _ in lens]
+        for s, p, m in zip(seqs, at, lens):
+            pool.seq_reserve(s, p + 2 * m + 1)
+            if p:
+                fill(tw, s, p, rng)
+        ks, vs = ([rows_of(rng, m, 2) for m in lens] for _ in range(2))
+        tw.append(0, seqs, at, ks, vs)
+        tw.assert_pools_equal()
+        bufs = [DeviceBuffer.from_numpy(np.concatenate(x)) for x in (ks, vs)] + [DeviceBuffer.from_numpy(x) for x in (gamma, table)]
+        behind = [p + m for p, m in zip(at, lens)]
+        pool.append_kprep(0, seqs, behind, lens, bufs[0], bufs[1], bufs[2], 1e-6, bufs[3], 64, 8192)
+        device_sync()
+        for s, p, m, k, v in zip(seqs, behind, lens, ks, vs):
+            if m:
+                tok = (p + np.arange(m)).astype(np.int32)
+                tw.images[0].append(pool.block_table(s), p, oracle.k_prep(k, 2, 256, gamma, 1e-6, table, 64, tok), v)
+        tw.assert_pools_equal()
+        total = sum(lens)
+        ko, vo = DeviceBuffer(total * 2048), DeviceBuffer(total * 2048)
+        pool.read_rows(0, seqs, behind, lens, ko, vo)
+        want = [np.concatenate(w) for w in zip(*[tw.images[0].gather(pool.block_table(s), p, m) for s, p, m in zip(seqs, behind, lens)])]
+        for got, w in zip((ko, vo), want):
+            assert np.array_equal(got.download(np.float32).reshape(w.shape), w)
+        for x in bufs + [ko, vo]:
+            x.free()
+
+
+@pytest.mark.parametrize("layout, hd, n_kv", [(L.LAYOUT_F16, 32, 1), (L.LAYOUT_F16, 256, 2), (L.LAYOUT_Q8V, 64, 3), (L.LAYOUT_I8H, 256, 1)])
+@pytest.mark.parametrize("n", [9, 40])
+def test_reading_back_very_different_lengths(layout, hd, n_kv, n):
+    rng = rng_of(41, layout, hd, n)
+    lens = [0, 1, 0, 0, 300, 1, 1, 0, 33] + [int(x) for x in rng.integers(0, 3, max(n - 11, 0))] + [19, 0][:max(n - 9, 0)]
+    with Pool(n_pages=200, n_kv_head=n_kv, head_dim=hd, layout=layout, max_seqs=n) as pool:
+        pool.set_free_order(rng.permutation(200).astype(np.int32))
+        seqs = [pool.seq_create() for _ in lens]
+        for s, m in zip(seqs, lens):
+            pool.seq_reserve(s, m + 3)
+        rows = [rng.standard_normal((sum(lens) + 3 * n, n_kv, hd)).astype(np.float32) for _ in range(2)]
+        kd, vd = (DeviceBuffer.from_numpy(x) for x in rows)
+        pool.append(0, seqs, [0] * n, [m + 3 for m in lens], kd, vd)
+        total = sum(lens)
+        ko, vo = DeviceBuffer(total * n_kv * hd * 4), DeviceBuffer(total * n_kv * hd * 4)
+        pool.read_rows(0, seqs, [2] * n, lens, ko, vo)
+        want = [np.concatenate(w) for w in zip(*[pool.gather(0, s, 2, m) for s, m in zip(seqs, lens) if m])]
+        for got, w in zip((ko, vo), want):
+            assert np.array_equal(got.download(np.float32).reshape(w.shape), w)
+        for x in (kd, vd, ko, vo):
+            x.free()
