@@ -1310,6 +1310,7 @@ bkv_status bkv_step_plan_decode(bkv_step_plan* pl, int32_t layer, const float* k
     if (ord != BKV_OK) return ord;
     AttnBatch b{};
     b.n = pl->n;
+    for (int i = 0; i < pl->n; ++i) b.pos[i] = (int32_t)pl->first[i];  // where the plan began: for what goes by size alone
     AttnArgs a;
     a.n_q_head = pl->n_q_head;
     a.q = q_dev;

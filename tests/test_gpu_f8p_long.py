@@ -6,7 +6,7 @@ import pytest
 import f8p_model as M
 import oracle
 from breccia_amd import lib as L
-from breccia_amd.kv import DeviceBuffer, Graph, Pool, Stream, device_sync, rope_table
+from breccia_amd.kv import DeviceBuffer, Graph, Pool, StepPlan, Stream, device_sync, rope_table
 from gpu_common import REF_BAR_MAX_REL, check_attn
 from test_gpu_f8p import cells_at, chunk, fill, lists, rng_of, rows_of
 
@@ -303,3 +303,33 @@ def test_reading_back_very_different_lengths(layout, hd, n_kv, n):
             assert np.array_equal(got.download(np.float32).reshape(w.shape), w)
         for x in (kd, vd, ko, vo):
             x.free()
+
+
+def test_a_captured_plan_of_long_walks_replays_eager_steps():
+    # 64 layers: pages go past the caches in the plan's launches as in the eager ones
+    lens, n_q, layer, n_tok = [1500, 700, 33], 16, 63, 6
+    assert sum(lens) * 2 * 512 * 64 >= 96 << 20
+    with M.F8Twin(n_layers=64, n_pages=160) as a, M.F8Twin(n_layers=64, n_pages=160) as b:
+        for tw in (a, b):
+            seqs = [tw.pool.seq_create() for _ in lens]
+            for s, n in zip(seqs, lens):
+                fill(tw, s, n, rng_of(42, s), layer)
+                tw.pool.seq_reserve(s, n + n_tok)
+        rng, st = rng_of(43), Stream()
+        kd, vd, qd, od = DeviceBuffer(3 * 2048), DeviceBuffer(3 * 2048), DeviceBuffer(3 * n_q * 1024), DeviceBuffer(3 * n_q * 1024)
+        plan = StepPlan(a.pool, seqs, lens, n_tok, n_q, st)
+        st.sync()
+        graph = Graph(st)
+        plan.decode(layer, kd, vd, qd, od, 1 / 16.0, stream=st)
+        plan.advance(st)
+        graph.end()
+        for t in range(n_tok):
+            q = rng.standard_normal((3, n_q, 256)).astype(np.float32)
+            kd.upload(rows_of(rng, 3, 2), st), vd.upload(rows_of(rng, 3, 2), st), qd.upload(q, st)
+            graph.launch()
+            got = od.download(np.float32, stream=st)
+            b.pool.decode_step(layer, seqs, [n + t for n in lens], kd, vd, n_q, qd, od, 1 / 16.0, stream=st)
+            assert np.array_equal(got, od.download(np.float32, stream=st)), t
+        assert np.array_equal(a.pool.read_layer(layer, 0), b.pool.read_layer(layer, 0))
+        graph.destroy()
+        plan.destroy()

@@ -6,7 +6,7 @@ import pytest
 from test_host_registers import compiled, scratch_of_kernels
 
 
-@pytest.mark.parametrize("source, kernels", [("f8p_decode.hip", 7), ("f8p_move.hip", 33)])
+@pytest.mark.parametrize("source, kernels", [("f8p_decode.hip", 8), ("f8p_move.hip", 33)])
 def test_nothing_spills(source, kernels):
     scratch = {k: int(v) for k, v in scratch_of_kernels(source).items()}
     assert len(scratch) == kernels, sorted(scratch)
