@@ -3,18 +3,22 @@
 //
 //   S^T[cell][row] = K[cell][:] . Q[row][:]      v_mfma_f32_16x16x32_f16, A = K (codes as f16, exact), B = q
 //   z              = S^T * 2^(e_K) + e_V          base-2 logits plus the exponent of the page's V
-//   w              = exp2(z - M)                  M: a running maximum of z, moved when it is passed by more than kF8Slack
+//   w              = exp2(z - M)                  M: kF8Lift below a running maximum of z, moved when that is passed by more than kF8Slack
 //   O^T[d][row]   += V^T[d][cell] . w[cell][row]  A = V (codes as f16, exact), 32 cells of two pages a product
 //   l             += w * 2^(-e_V)
 //
-// So the scale of K is a factor of the page's scores and that of V rides on the weights: the largest terms have weights near 1
+// So the scale of K is a factor of the page's scores and that of V rides on the weights: the largest terms have the largest weights
 // whatever the magnitude of their values, pages of different scales meet in one product, and out = O / l with both relative to
-// M.  Exponents lie in -32 .. 31, which keeps the terms of l below 2^(kF8Slack + 32 + log2 of the cells) and its largest one
-// above 2^-70.
+// M.  Exponents lie in -32 .. 31, which keeps the terms of l below 2^(kF8Lift + kF8Slack + 32 + log2 of the cells) and its largest one
+// at 2^(kF8Lift - 31) or more.
 //
-// q and the weights enter as the sum of two f16 numbers (two products each): 22 bits and more.  q's row is brought to a largest
-// value of 2^13 .. 2^14 first, by a power of two that rejoins the scale of K: neither part leaves what f16 can hold, whatever the
-// queries' size.  The sums are f32, in the matrix cores.
+// q and the weights enter as the sum of two f16 numbers (two products each).  q's row is brought to a largest value of 2^13 .. 2^14 first,
+// by a power of two that rejoins the scale of K: neither part leaves what f16 can hold, whatever the queries' size, and an element is
+// off by 2^-22 of itself and 2^-38 of the row's largest.  A weight is off by 2^-22 of itself or by 2^-25: f16's steps end there.
+// The largest term's is 2^kF8Lift .. 2^(kF8Lift + kF8Slack), as far up as f16 reaches, so a term is off by 2^-22 of itself and 2^-34
+// of the largest one.  (M at the maximum itself made the latter 2^-25: a chunk's 8000 equal weights behind a key that brings nothing,
+// 19.7 bits above them, were off by 1.5e-2 of the output, 25.6 bits above them they were lost; now 7e-5 and 6e-4, in the same
+// time.)  The sums are f32, in the matrix cores.
 //
 // A lane (c = lane % 16, g = lane / 16) holds of a tile row c, and cells 4 g .. 4 g + 3 of either page: weights come out of the
 // softmax in the order the second product takes them in.
@@ -31,7 +35,7 @@ typedef _Float16 f8_h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f8_h2 __attribute__((ext_vector_type(2)));
 typedef float f8_f4 __attribute__((ext_vector_type(4)));
 
-constexpr float kF8Slack = 6.0f;
+constexpr float kF8Lift = 9.0f, kF8Slack = 6.0f;  // 2^15 at most: f16 ends at 65504
 
 __device__ __forceinline__ f8_f4 f8_mfma(f8_h8 a, f8_h8 b, f8_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 

@@ -333,7 +333,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
         const auto has_dead = [&](int u) { return (first_pg + u + 2) * kPage - 1 > all_live || u + 1 >= mine; };
         // the first of the lane's cells of page p of pair u; past the end one that nobody attends
         const auto cell_of = [&](int u, int p) { return u + p < mine ? (first_pg + u + p) * kPage + 4 * g : 0x7fffff00; };
-        // dead cells out of pair u, and M moved where the pair passes it by more than kF8Slack
+        // dead cells out of pair u, and M moved where the pair passes it by more than kF8Lift + kF8Slack
         const auto move_reference = [&](int u) {
             if (has_dead(u)) {
 #pragma unroll
@@ -358,8 +358,8 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                 for (int t = 0; t < TILES; ++t) {
                     // (nothing attended yet: nothing to keep, whatever the exponential of it would be)
                     const bool moved = pm[t] > limit[t];
-                    const float up = moved ? pm[t] : 0.0f, keep = limit[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
-                    limit[t] = moved ? kF8Slack : limit[t];
+                    const float up = moved ? pm[t] - kF8Lift : 0.0f, keep = limit[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                    limit[t] = moved ? kF8Lift + kF8Slack : limit[t];
                     at[t] += up;
                     l_run[t] *= keep;
 #pragma unroll

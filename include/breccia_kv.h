@@ -251,7 +251,8 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  *   K   1024 (c / 4) + 64 (8 (d / 128) + d / 4 % 8) + 16 (c % 4) + 4 (d / 32 % 4) + d % 4
  *   V   1024 (c / 4) + 4 d + c % 4
  * Exponents read from a page are brought into -32 .. 31.  A NaN in a row that a query attends makes NaN of what the query gets
- * from it (K: the whole output row; V: its element), and of nothing else. */
+ * from it (K: the whole output row; V: its element), and of nothing else.  Attention weighs a cell's V to 2^-22 of itself and 2^-34 of
+ * the largest of the row's weights (weights of V as stored: times 2^e of V's page), decode and chunks alike. */
 
 /* ---- hot path ---------------------------------------------------------------
  * bkv_append replaces Qsa::kv_append + shaders/qsa_kv_append.comp (qsa/mod.rs:
@@ -347,8 +348,9 @@ bkv_status bkv_decode_attn_static(bkv_pool *pool, int32_t layer, int32_t n, cons
  * sequence seqs[i].  The chunk's own K/V must have been appended first.  q, out: device f32
  * [sum n_tokens][n_q_head][head_dim], chunks concatenated in call order; gate(token, h, d) =
  * gate_dev[token*gate_tok_stride + h*gate_head_stride + d] or NULL.  K and V enter the MFMAs
- * as the exact f16 the cache holds; q and the probabilities are f32 split into two f16 parts,
- * so accuracy is that of f32 accumulation.  q8_0 V blocks (BRECCIA_KV_Q8V in
+ * as the exact f16 the cache holds; q and the probabilities are f32 split into two f16 parts, the
+ * sums are f32: a probability is off by 2^-22 of itself and 2^-25 (e4m3 pages: 2^-34) of the row's
+ * largest.  q8_0 V blocks (BRECCIA_KV_Q8V in
  * qsa_attn_apply_gqa.comp:53-77) are dequantised once per work-group into two f16 terms whose
  * sum carries code * scale to 22 bits, and so are int8 K blocks; e4m3 codes are f16 numbers, their
  * scales join the scores and the weights.  All layouts, head_dim 256, 16-cell pages.  Written
