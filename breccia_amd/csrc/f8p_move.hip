@@ -2,8 +2,8 @@
 //
 // Written rows join a page under one scale with the rows below them that it holds already.  So a work-group has a whole unit,
 // K or V of a (page, kv head): it holds all 16 rows in registers, 16 values a thread, agrees on the largest magnitude, and
-// writes all codes.  Rows behind the last one written are cleared: what a page holds follows from the rows written into it,
-// whoever had it before.  (K and V in one work-group: five ragged chunks of 2073 rows at n_kv = 4 9.5 us, apart 8.7.)
+// writes all codes.  Rows behind the last one written are cleared: of what others left in a page nothing counts that lies behind a
+// written row.  (K and V in one work-group: five ragged chunks of 2073 rows at n_kv = 4 9.5 us, apart 8.7.)
 //
 // Everything here moves bytes.  Small calls take what a launch and two dependent trips to memory take, 3.5 us; reading back
 // 131072 cells as binary16, 402 MB, takes 67 us, 6.0 TB/s, what a copy reaches here.

@@ -239,11 +239,17 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  *          (31 where none is)
  *   code   x * 2^-e rounded to nearest, ties to even; beyond +-448 the largest code; NaN for NaN and infinities
  *   value  code * 2^e
- * A write (bkv_append, _f16, _kprep; bkv_decode_step and step plans too) touches whole pages.  In a page that holds cells below
- * the first one written those keep their values, under the scale of all of the page's rows -- exactly, but for values that a larger
- * scale brings below 2^-6 * 2^e and which are rounded again, by at most 2^-10 * 2^e; cells behind the last one written are
+ * A write (bkv_append, _f16, _kprep; bkv_decode_step and step plans too) touches whole pages.  In the page of the first written
+ * cell the cells below it are read and coded again, under the scale of all of the page's rows; cells behind the last one written are
  * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, and two entries of
- * one call must not write the same page (BKV_ERR_INVALID).  What a page holds depends on the rows written into it alone.
+ * one call must not write the same page (BKV_ERR_INVALID).
+ * Coded again, a value is the same number unless the scale is larger than all that its page has had since it was written: then what
+ * falls below 2^-6 * 2^e is rounded again, by at most 2^-10 * 2^e.  That stays, whatever becomes of the rows that made the scale:
+ * what a page holds depends on the writes into it one after the other, rows taken back since (bkv_seq_truncate) among them.  A
+ * finite value x of at most 448 * 2^31 is held to 2^-4 |x| + 2^-9 * 2^E, E the largest exponent that its page, kv head and side have
+ * had since it was written.  A caller that writes rows which it may take back, and that are far larger than those below them, keeps these as
+ * they were by writing into a fork (bkv_seq_fork: the child's reserve gives it a copy of the page).  Cells below the first written one
+ * of a page that nobody has written (a write into the middle of a fresh page) count as what the page held for others before.
  * bkv_decode_step, and a step plan's decode, are the write's launch and then the attention's.  A call writes fewer than 2^23 pages
  * x kv heads (BKV_ERR_INVALID otherwise).
  * A K page is n_kv_head units of 4096 bytes and a line of 128 with the exponents, int32 [kv head][K, V]; a V page n_kv_head units.
