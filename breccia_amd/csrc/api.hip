@@ -1070,8 +1070,15 @@ static bkv_status decode_attn_common(bkv_pool* p, int32_t layer, int32_t n, cons
         a.id_stride = id_stride;
         a.max_ids = max_ids;
     }
+    // the pool's own workspace is ordered across streams; the static scratch is the device's, shared by
+    // every pool, and overlapping calls on it are the caller's to avoid
+    if (!static_ws) {
+        st = order_workspace(p->attn_ws, S(stream));
+        if (st != BKV_OK) return st;
+    }
     if (step && p->g.layout == BKV_LAYOUT_F8P) {
-        // a new row changes its page's scale, and with it the page: a launch ahead of the attention
+        // The new row goes in with a launch of its own, once nothing can fail any more: it may change the scale of its page, and the
+        // attention kernel does not code pages.
         AppendBatch rows{};
         rows.n = n;
         for (int i = 0; i < n; ++i) rows.row[i] = b.row[i], rows.pos0[i] = b.pos[i], rows.n_tok[i] = 1, rows.src0[i] = i;
@@ -1079,12 +1086,6 @@ static bkv_status decode_attn_common(bkv_pool* p, int32_t layer, int32_t n, cons
     } else if (step) {
         a.new_k = new_k_dev;
         a.new_v = new_v_dev;
-    }
-    // the pool's own workspace is ordered across streams; the static scratch is the device's, shared by
-    // every pool, and overlapping calls on it are the caller's to avoid
-    if (!static_ws) {
-        st = order_workspace(p->attn_ws, S(stream));
-        if (st != BKV_OK) return st;
     }
     BKV_HIP(launch_decode_attn(p, layer, b, a, S(stream)));
     return BKV_OK;
