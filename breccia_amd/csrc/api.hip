@@ -1093,6 +1093,13 @@ static bkv_status decode_attn_common(bkv_pool* p, int32_t layer, int32_t n, cons
 
 bkv_status bkv_attn_plan(int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int32_t n, const int64_t* pos,
                          int32_t sel_groups, int32_t* splits_out, int32_t* pps_out, int32_t* total_out) {
+    return bkv_attn_plan_layout(BKV_LAYOUT_F16, n_cu, n_kv_head, n_q_head, n, pos, sel_groups, splits_out, pps_out, total_out);
+}
+
+bkv_status bkv_attn_plan_layout(int32_t layout, int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int32_t n, const int64_t* pos,
+                                int32_t sel_groups, int32_t* splits_out, int32_t* pps_out, int32_t* total_out) {
+    if (layout < BKV_LAYOUT_F16 || layout > BKV_LAYOUT_F8P)
+        return fail(BKV_ERR_INVALID, sfmt("attn_plan: unknown layout %lld", layout));
     if (n_cu <= 0 || n_kv_head <= 0 || n_kv_head > BKV_MAX_KV_HEAD)
         return fail(BKV_ERR_INVALID, sfmt("attn_plan: %lld compute units, %lld kv heads", n_cu, n_kv_head));
     if (n_q_head <= 0 || n_q_head % n_kv_head != 0 || n_q_head / n_kv_head > BKV_MAX_HEAD_GROUP)
@@ -1108,7 +1115,7 @@ bkv_status bkv_attn_plan(int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int3
             return fail(BKV_ERR_RANGE, sfmt("attn_plan: position %lld of entry %lld", pos[i], i));
         b.pos[i] = (int32_t)pos[i];
     }
-    const AttnPlanLimits lim = attn_plan_limits(n_cu, kMaxWgs, n_kv_head, n_q_head / n_kv_head, BKV_LAYOUT_F16);
+    const AttnPlanLimits lim = attn_plan_limits(n_cu, kMaxWgs, n_kv_head, n_q_head / n_kv_head, layout);
     const int32_t total = plan_attn_ranges(lim, 16, sel_groups, b);
     if (total < 0)
         return fail(BKV_ERR_INVALID, sfmt("attn_plan: %lld entries x %lld kv heads need more work-groups than "

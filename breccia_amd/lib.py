@@ -104,6 +104,7 @@ _SIGNATURES = {
     "bkv_decode_attn_static": (C.c_int, [_vp, _i32, _i32, _pi32, _pi64, _i32, _vp, _vp, _i64, _i64, _f32,
                                          _vp, _vp]),
     "bkv_attn_plan": (C.c_int, [_i32, _i32, _i32, _i32, _pi64, _i32, _pi32, _pi32, _pi32]),
+    "bkv_attn_plan_layout": (C.c_int, [_i32, _i32, _i32, _i32, _i32, _pi64, _i32, _pi32, _pi32, _pi32]),
     "bkv_prefill_attn": (C.c_int, [_vp, _i32, _i32, _pi32, _pi64, _pi32, _i32, _vp, _vp, _i64, _i64, _f32,
                                    _vp, _vp]),
     "bkv_decode_step": (C.c_int, [_vp, _i32, _i32, _pi32, _pi64, _vp, _vp, _i32, _vp, _vp, _i64, _i64, _f32,

@@ -569,17 +569,20 @@ bkv_status bkv_read_rows(bkv_pool *pool, int32_t layer, int32_t n_seqs, const in
 bkv_status bkv_read_rows_f16(bkv_pool *pool, int32_t layer, int32_t n_seqs, const int32_t *seqs, const int64_t *cell0,
                              const int32_t *n_cells, uint16_t *k_out_dev, uint16_t *v_out_dev, void *stream);
 
-/* How a decode-attention batch would be cut into work-groups on a device of n_cu compute units (on a
- * BKV_LAYOUT_F8P pool ranges are multiples of eight pages instead of four):
+/* How a decode-attention batch would be cut into work-groups on a device of n_cu compute units:
  * the planning step of bkv_decode_attn / bkv_decode_step / bkv_decode_attn_select alone, on the
  * host, nothing launched (no pool or device needed).  pos[n] as for those calls; sel_groups > 0
  * plans every entry for that many groups of four listed blocks (a selection list of
  * 4 * sel_groups ids) instead of its pages.  splits_out[n], pps_out[n]: page ranges per entry and
  * pages per range; *total_out: work-groups of the launch.  BKV_ERR_INVALID when the batch needs
  * more work-groups than the partial-result workspace holds -- the error the attention calls
- * themselves return, before anything is enqueued (qsa/mod.rs:1108-1116). */
+ * themselves return, before anything is enqueued (qsa/mod.rs:1108-1116).
+ * _layout: on a pool of that layout (ranges are multiples of eight pages on BKV_LAYOUT_F8P, of four on the
+ * others); bkv_attn_plan is that of BKV_LAYOUT_F16. */
 bkv_status bkv_attn_plan(int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int32_t n, const int64_t *pos,
                          int32_t sel_groups, int32_t *splits_out, int32_t *pps_out, int32_t *total_out);
+bkv_status bkv_attn_plan_layout(int32_t layout, int32_t n_cu, int32_t n_kv_head, int32_t n_q_head, int32_t n, const int64_t *pos,
+                                int32_t sel_groups, int32_t *splits_out, int32_t *pps_out, int32_t *total_out);
 
 /* ---- per-kernel GPU timing ------------------------------------------------------
  * The analogue of Qsa::stage_timings / Pipe::run_timed (qsa/mod.rs:1733-1970,
