@@ -37,6 +37,10 @@ typedef float f8_f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kF8Lift = 9.0f, kF8Slack = 6.0f;  // 2^15 at most: f16 ends at 65504
 
+// 2^up for the elements of a row of q; NaN where the scale of the logits is not finite.  (Where that scale is used it is kept
+// finite, and a NaN would not come through.)
+__device__ __forceinline__ float f8_lift_q(int up, float scale_log2e) { return exp2_int(up) + (scale_log2e - scale_log2e); }
+
 __device__ __forceinline__ f8_f4 f8_mfma(f8_h8 a, f8_h8 b, f8_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // 4 + 4 codes as f16 numbers; the conversion is exact (e4m3's subnormals are f16 normals), NaN stays NaN

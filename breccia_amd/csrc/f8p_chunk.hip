@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
             }
             top = max_over_lane_groups(top);
             const int up = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -126), 126);
-            const float by = exp2_int(up);
+            const float by = f8_lift_q(up, P.scale_log2e);
             down[t] = exp2_int(-up) * P.scale_log2e;
 #pragma unroll
             for (int f = 0; f < 8; ++f)

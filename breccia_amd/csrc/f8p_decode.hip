@@ -49,7 +49,7 @@ struct Walk {
             for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(raw[f][j >> 2][j & 3]));
         top = max_over_lane_groups(top);
         const int up = min(max(13 - ((int)(__float_as_uint(top) >> 23) - 127), -126), 126);
-        const float by = exp2_int(up);
+        const float by = f8_lift_q(up, scale_log2e);
         down = exp2_int(-up) * scale_log2e;
 #pragma unroll
         for (int f = 0; f < 8; ++f)

@@ -258,7 +258,8 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  *   V   1024 (c / 4) + 4 d + c % 4
  * Exponents read from a page are brought into -32 .. 31.  A NaN in a row that a query attends makes NaN of what the query gets
  * from it (K: the whole output row; V: its element), and of nothing else.  Attention weighs a cell's V to 2^-22 of itself and 2^-34 of
- * the largest of the row's weights (weights of V as stored: times 2^e of V's page), decode and chunks alike. */
+ * the largest of the row's weights (weights of V as stored: times 2^e of V's page), decode and chunks alike.  A scale of the logits
+ * that is not finite makes NaN of all outputs. */
 
 /* ---- hot path ---------------------------------------------------------------
  * bkv_append replaces Qsa::kv_append + shaders/qsa_kv_append.comp (qsa/mod.rs:
