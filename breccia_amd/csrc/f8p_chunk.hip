@@ -100,16 +100,7 @@ __device__ __forceinline__ ChunkUnit chunk_unit(const std::conditional_t<SPLIT, 
 }
 
 __device__ __forceinline__ int wave_value(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// keeps a value where it is computed: between matrix products, not behind the branch that its use stands behind
-template <typename T>
-__device__ __forceinline__ void stay(T& x) {
-    asm volatile("" : "+v"(x));
-}
 __device__ __forceinline__ unsigned lds_at(const float* p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) float*)p; }
-// two f32 numbers as f16, rounded to nearest
-__device__ __forceinline__ f8_h2 f8_pair(float a, float b) { return __builtin_convertvector(f8_f2{a, b}, f8_h2); }
-// x - (the f16 number hi), in one instruction that takes hi as it is (minus_one: -1.0f that the compiler cannot see through)
-__device__ __forceinline__ float f8_rest(float x, _Float16 hi, float minus_one) { return __builtin_fmaf((float)hi, minus_one, x); }
 // a maximum whose operands are known not to be signalling NaNs; fmaxf would quiet each of them first
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float x;
@@ -286,8 +277,8 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
 #pragma unroll
                 for (int j = 0; j < 8; j += 2) {
                     const float a = raw[f][j >> 2][j & 3] * by, b = raw[f][j >> 2][(j & 3) + 1] * by;
-                    const f8_h2 hi = f8_pair(a, b);
-                    const f8_h2 lo = f8_pair(f8_rest(a, hi[0], minus_one), f8_rest(b, hi[1], minus_one));
+                    const f8_h2 hi = to_f16(a, b);
+                    const f8_h2 lo = to_f16(remainder_of(a, hi[0], minus_one), remainder_of(b, hi[1], minus_one));
                     qhi[t][f][j] = hi[0], qhi[t][f][j + 1] = hi[1];
                     qlo[t][f][j] = lo[0], qlo[t][f][j + 1] = lo[1];
                 }
@@ -429,8 +420,8 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                     const int t = (part - 4) >> 2, r = 2 * ((part - 4) & 3);
                     sum[t][r >> 2] += z[t][r];
                     sum[t][r >> 2] += z[t][r + 1];
-                    f8_h2 hi = f8_pair(z[t][r], z[t][r + 1]);
-                    f8_h2 lo = f8_pair(f8_rest(z[t][r], hi[0], minus_one), f8_rest(z[t][r + 1], hi[1], minus_one));
+                    f8_h2 hi = to_f16(z[t][r], z[t][r + 1]);
+                    f8_h2 lo = to_f16(remainder_of(z[t][r], hi[0], minus_one), remainder_of(z[t][r + 1], hi[1], minus_one));
                     stay(hi), stay(lo);
                     ph[t][r] = hi[0], ph[t][r + 1] = hi[1];
                     pl[t][r] = lo[0], pl[t][r + 1] = lo[1];

@@ -7,7 +7,6 @@
 // take them, so they go straight to registers, 16 KiB a wave in flight, the next pair asked for as soon as the last use of this
 // one's is behind.  Sixteen contexts of 8k to 128k, 1.41 GB: 222 us, 6.4 TB/s of the 6.8 that a plain read reaches; short ones are
 // 9 us of start, fold and merge.
-#include <algorithm>
 #include <type_traits>
 
 #include "decode_attn_common.hpp"
@@ -339,7 +338,7 @@ hipError_t launch_decode_attn_f8p(const AttnKernelParams& kp, const AttnBatch& b
         else hipLaunchKernelGGL(kernel, dim3((unsigned)total), dim3(kBlock), 0, stream, args);
     };
     int64_t cells = 0;
-    for (int i = 0; i < b.n; ++i) cells += sel ? std::min<int64_t>(b.pos[i] + 1, 4ll * kp.max_ids) : b.pos[i] + 1;
+    for (int i = 0; i < b.n; ++i) cells += b.pos[i] + 1;
     const bool once = cells * kp.n_kv * 2 * kF8Hd * n_layers >= kOnceFrom;
     if (kp.bd) {
         // (the device's positions are a plan's; b has those that it began with)

@@ -65,7 +65,6 @@ struct F8Share {
         v_at = w * 1024 + l * 16;
     }
 };
-__device__ __forceinline__ void transpose4x4(const unsigned (&w)[4], unsigned (&t)[4]) { transpose4x4_bytes(w, t); }
 
 // One half (K or V) of a unit that lies in registers, x[u]: K's elements k_col + 32 u .., V's row v_row + u, coded and stored.
 // Rows below `kept` are in the page and come from `old` (loaded by the caller) under their old scale, rows from `end` on are
@@ -81,7 +80,7 @@ __device__ __forceinline__ void settle_rows(const F8Share& at, float (&x)[4][4],
     if (kept > 0) {
         const float scale = exp2_int(old.e);
         unsigned in[4] = {old.w.x, old.w.y, old.w.z, old.w.w}, rows[4];
-        if constexpr (V) transpose4x4(in, rows);
+        if constexpr (V) transpose4x4_bytes(in, rows);
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             if (row(u) < kept) f8p_values4(V ? rows[u] : in[u], scale, x[u]);
@@ -104,7 +103,7 @@ __device__ __forceinline__ void store_codes(const F8Share& at, const float (&x)[
     unsigned codes[4], out[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) out[u] = codes[u] = f8p_codes4(x[u], by);
-    if constexpr (V) transpose4x4(codes, out);
+    if constexpr (V) transpose4x4_bytes(codes, out);
     *reinterpret_cast<v4u*>(unit + (V ? at.v_at : at.k_at)) = v4u{out[0], out[1], out[2], out[3]};
     if (tid == 0) *exponent = e;
 }
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(kBlock) void read_rows_f8p_kernel(Batch b, F8MoveGe
     };
     const float ks = exp2_int(k.e), vs = exp2_int(v.e);
     unsigned cols[4] = {v.w.x, v.w.y, v.w.z, v.w.w}, rows[4];
-    transpose4x4(cols, rows);
+    transpose4x4_bytes(cols, rows);
     if constexpr (std::is_same<DstT, uint16_t>::value) {
         // Two lanes have neighbouring fours: the even one takes both fours of the even dwords, the odd one of the odd dwords, and
         // stores are 16 bytes a lane, whole 128-byte lines an instruction.

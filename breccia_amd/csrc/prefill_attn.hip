@@ -110,21 +110,6 @@ __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
     lo = (_Float16)(x - (float)hi);
 }
 
-// two f32 numbers as f16, rounded to nearest
-__device__ __forceinline__ h2m to_f16(float a, float b) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    return __builtin_convertvector(f2{a, b}, h2m);
-}
-// x - (the f16 number hi): one v_fma_mix_f32 takes the f16 operand as it is (minus_one: -1.0f that the compiler
-// cannot see through, a plain subtraction would be preceded by a conversion)
-__device__ __forceinline__ float remainder_of(float x, _Float16 hi, float minus_one) {
-    return __builtin_fmaf((float)hi, minus_one, x);
-}
-// keeps a value where it is computed: between matrix products, not behind the branch that its use stands behind
-template <typename T>
-__device__ __forceinline__ void stay(T& x) {
-    asm volatile("" : "+v"(x));
-}
 // a maximum whose operands are known not to be signalling NaNs; fmaxf would quiet each of them first
 __device__ __forceinline__ float max_of(float a, float b) {
     asm("v_max_f32 %0, %0, %1" : "+v"(a) : "v"(b));

@@ -73,6 +73,23 @@ __device__ __forceinline__ uint64_t lane_value(uint64_t x, int i) {
     return (uint64_t)hi << 32 | lo;
 }
 
+// two f32 numbers as f16, rounded to nearest
+typedef _Float16 f16_pair __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ f16_pair to_f16(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_convertvector(f2{a, b}, f16_pair);
+}
+// x - (the f16 number hi): one v_fma_mix_f32 takes the f16 operand as it is (minus_one: -1.0f that the compiler
+// cannot see through, a plain subtraction would be preceded by a conversion)
+__device__ __forceinline__ float remainder_of(float x, _Float16 hi, float minus_one) {
+    return __builtin_fmaf((float)hi, minus_one, x);
+}
+// keeps a value where it is computed: between matrix products, not behind the branch that its use stands behind
+template <typename T>
+__device__ __forceinline__ void stay(T& x) {
+    asm volatile("" : "+v"(x));
+}
+
 typedef const __attribute__((address_space(1))) uint8_t* page_ptr;  // said to be global memory: its address goes through integers
 // 16 bytes a lane straight into LDS: lane l's go to byte lds + 16 l.  Nothing but the vector-memory count says when they
 // have landed; each wave waits for its own ahead of the barrier that publishes them.
