@@ -1422,7 +1422,7 @@ bkv_status bkv_prefill_attn(bkv_pool* p, int32_t layer, int32_t n_seqs, const in
             return fail(BKV_ERR_INVALID, "prefill_attn: more than 2^24 tokens in one call");
     }
     b.n = n_seqs;
-    // e4m3 pages take blocks and cuts like f16 ones: one or two tiles of rows a wave
+    // e4m3 pages take blocks and cuts like f16 ones: one or two tiles of rows a wave (what that gives there: prefill_plan.hpp)
     const bool f16 = p->g.layout == BKV_LAYOUT_F16 || p->g.layout == BKV_LAYOUT_F8P;
     const int64_t rows_per_wg = prefill_rows_per_wg(f16, wgs, p->n_cu);
     order_chunks(b, p->g.n_kv, (int32_t)group, (int32_t)rows_per_wg);

@@ -580,6 +580,7 @@ hipError_t launch_chunk_attn_f8p(bkv_pool* p, const PrefillSplitParams& kp, int3
         else launch(chunk_attn_f8p_kernel<1, false>, whole);
         return hipGetLastError();
     }
+    // (a call is cut while it leaves half of the compute units idle, and takes two tiles from two work-groups a unit on: not both)
     if (two) launch(chunk_attn_f8p_kernel<2, true>, kp);
     else launch(chunk_attn_f8p_kernel<1, true>, kp);
     const hipError_t err = hipGetLastError();

@@ -39,7 +39,7 @@ struct PrefillSplit {
 };
 
 struct PrefillPlanLimits {
-    bool f16;      // the layout: f16 pools, or quantised ones
+    bool f16;      // the layout: f16 and e4m3 pools, or q8_0 V and int8 ones
     int32_t n_kv;
     int32_t n_cu;
     int64_t rows;  // query rows a workspace holds partial results for
@@ -109,6 +109,10 @@ BKV_HD inline int split_ranges(int pages, int pps, int max_splits, int& each) {
 // Query rows one work-group of four waves owns, in tiles of 16: two tiles a wave or one.  f16 pools: 128 when the chunks
 // make more 64-row work-groups than fit the chip at two per compute unit (then sharing the page images among more rows is
 // worth more than spreading out), else 64.
+// e4m3 pools go by the same rule, which was not made for their kernel.  What it does there, at 8 heads a kv head, two of these, us with
+// 64 rows / 128: one chunk behind 2000 cells 1500 tokens 146 / 163, 2040 190 / 193, 2056 (the first that takes 128) 215 / 210, 2600 261 / 259;
+// 4096 from scratch 250 / 226.  128 lose where they leave a second round of work-groups nearly empty: 2056 from scratch 84 / 103, four
+// chunks of 600 behind 1500 each 152 / 166.
 inline int32_t prefill_rows_per_wg(bool f16, int64_t wgs_of_64_rows, int32_t n_cu) {
     if (!f16) return 8 * kPrefillRowsPerWave;
     return wgs_of_64_rows > 2 * (int64_t)(n_cu > 0 ? n_cu : 256) ? 8 * kPrefillRowsPerWave : 4 * kPrefillRowsPerWave;
@@ -157,6 +161,11 @@ inline int32_t last_done(const std::vector<int32_t>& runs, int32_t units) {
 // us, uncut / cut: 41 tokens behind 517 cells 24.2 / 15.0, 100 behind 8000 249 / 43, 200 behind 3000 with q8_0 V 214 / 48,
 // 300 behind 1000 on an int8 pool 103 / 39, 900 behind 2000 218 / 130; two chunks of 530 q8_0 V 48 / 39 (int8 52 / 41), 1900
 // from scratch 134 / 123 (148 / 130), 400 with 48 heads 40 / 37 (44 / 38), two of 530 behind 700 92 / 87 (101 / 92).
+// e4m3 pools are cut by the f16 ratios, which were not fitted to their kernel.  us there, uncut / cut, at 8 heads a kv head, two of these: 41
+// tokens behind 517 cells 21.2 / 13.9, 64 behind 2000 60 / 19, 100 behind 8000 278 / 44, 200 behind 2000 74 / 33, 400 behind 8000 296 / 112,
+// 400 from scratch 18.3 / 19.2, 300 behind 100 with 60 behind 8000 284 / 35.  Calls that keep more than half of the compute units busy
+// stay uncut, and take up to ten times their products' time where their chunks are very unequal: 30 tokens behind 8000 beside 700 from
+// scratch and 200 behind 3000 279 (products 29), 800 behind 8000 306 (177).
 // chain: page pairs of the cut call's longest chain, where it was worked out.
 inline bool plan_prefill_split(const PrefillPlanLimits& lim, const PrefillBatch& b, int32_t rows, int32_t group, PrefillSplit& s,
                                int32_t& chain) {
