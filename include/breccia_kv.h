@@ -143,7 +143,8 @@ bkv_status bkv_seq_free(bkv_pool *pool, int32_t seq);
 bkv_status bkv_seq_reserve(bkv_pool *pool, int32_t seq, int64_t new_len, bkv_page_pair *cow_pairs,
                            int32_t cow_capacity, int32_t *n_cow);
 /* Set the sequence's length without touching pages (speculative rollback:
- * rejected cells are simply overwritten later, docs/specs/qwen4exp-architecture.md:750-759). */
+ * rejected cells are simply overwritten later, docs/specs/qwen4exp-architecture.md:750-759; on
+ * BKV_LAYOUT_F8P the rows below them in their page keep what the rejected ones' scale cost, below). */
 bkv_status bkv_seq_truncate(bkv_pool *pool, int32_t seq, int64_t new_len);
 int64_t bkv_seq_len(const bkv_pool *pool, int32_t seq);           /* -1 on error */
 int64_t bkv_seq_capacity(const bkv_pool *pool, int32_t seq);      /* cells addressable */
@@ -241,8 +242,9 @@ bkv_status bkv_prefix_prefetch(bkv_pool *pool, const int32_t *tokens, int64_t n_
  *   value  code * 2^e
  * A write (bkv_append, _f16, _kprep; bkv_decode_step and step plans too) touches whole pages.  In the page of the first written
  * cell the cells below it are read and coded again, under the scale of all of the page's rows; cells behind the last one written are
- * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, and two entries of
- * one call must not write the same page (BKV_ERR_INVALID).
+ * cleared.  So of the cells of a sequence only those before a written one outlive the write within its page, two entries of one call
+ * must not write the same page (BKV_ERR_INVALID), and a write is ordered by the caller behind whatever still reads earlier cells of the page
+ * on another stream (bkv_decode_step orders itself behind the pool's decode calls before it, a step plan's decode behind the plan's).
  * Coded again, a value is the same number unless the scale is larger than all that its page has had since it was written: then what
  * falls below 2^-6 * 2^e is rounded again, by at most 2^-10 * 2^e.  That stays, whatever becomes of the rows that made the scale:
  * what a page holds depends on the writes into it one after the other, rows taken back since (bkv_seq_truncate) among them.  A
