@@ -36,6 +36,12 @@ typedef _Float16 f8_h2 __attribute__((ext_vector_type(2)));
 typedef float f8_f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kF8Lift = 9.0f, kF8Slack = 6.0f;  // 2^15 at most: f16 ends at 65504
+// Where M goes when it moves to a maximum.  (From 2^24 on f32 does not hold what lies kF8Lift below: from 2^27 it would be 16 below, and
+// weights past f16's end.)
+__device__ __forceinline__ float f8_reference(float top) {
+    const float at = top - kF8Lift;
+    return top - at > kF8Lift + kF8Slack ? top : at;
+}
 
 // 2^up for the elements of a row of q; NaN where the scale of the logits is not finite.  (Where that scale is used it is kept
 // finite, and a NaN would not come through.)

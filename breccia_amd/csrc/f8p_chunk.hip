@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256, TILES == 2 ? 1 : 2) void chunk_attn_f8p_kernel
                 for (int t = 0; t < TILES; ++t) {
                     // (nothing attended yet: nothing to keep, whatever the exponential of it would be)
                     const bool moved = pm[t] > limit[t];
-                    const float up = moved ? pm[t] - kF8Lift : 0.0f, keep = limit[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                    const float up = moved ? f8_reference(pm[t]) : 0.0f, keep = limit[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-up);
                     limit[t] = moved ? kF8Lift + kF8Slack : limit[t];
                     at[t] += up;
                     l_run[t] *= keep;

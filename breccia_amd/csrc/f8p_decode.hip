@@ -88,8 +88,8 @@ struct Walk {
         float pm = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])), fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
         pm = max_over_lane_groups(pm);
         const float was = m;
-        const bool moved = pm > m + (kF8Lift + kF8Slack);
-        m = moved ? pm - kF8Lift : m;
+        const bool moved = pm - m > kF8Lift + kF8Slack;  // (of sums with M the rounding could hide that)
+        m = moved ? f8_reference(pm) : m;
         const float at = m == -INFINITY ? 0.0f : m;  // nothing attended yet
         if (__builtin_amdgcn_ballot_w64(moved) != 0) {
             const float keep = __builtin_amdgcn_exp2f(was - at);
