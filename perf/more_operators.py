@@ -320,10 +320,6 @@ def prepare(case, seed):
 
     def write(pool, layer, seq, first, pair):
         if pair[0].shape[0]:
-            if layout == "i8":
-                # torch divides by a number as a product with its reciprocal, one scale in ten thousand rounds the other way: the rows
-                # that the plain form keeps, which are int8 rows as they are
-                pair = [_value(_hold(layout, rows), rows.shape[0]) for rows in pair]
             pool.append(layer, [seq], [first], [pair[0].shape[0]], pair[0].data_ptr(), pair[1].data_ptr())
 
     if kind == "shared":
