@@ -128,11 +128,17 @@ bkv_status ring_upload(bkv_pool* p, const void* host_src, size_t bytes, hipStrea
     return BKV_OK;
 }
 
-bkv_status ring_done(bkv_pool* p, int slot, hipStream_t stream) {
-    BKV_HIP(hipEventRecord(p->ring.ev[slot], stream));
-    p->ring.used[slot] = true;
+// An event behind what the stream has been given.  Where it cannot be recorded that work is waited for, and `recorded` is false: there is
+// nothing left to order behind.
+static bkv_status record_behind(hipEvent_t ev, hipStream_t stream, bool& recorded) {
+    recorded = hipEventRecord(ev, stream) == hipSuccess;
+    if (recorded) return BKV_OK;
+    (void)hipGetLastError();
+    BKV_HIP(hipDeviceSynchronize());
     return BKV_OK;
 }
+
+bkv_status ring_done(bkv_pool* p, int slot, hipStream_t stream) { return record_behind(p->ring.ev[slot], stream, p->ring.used[slot]); }
 
 // Pages on their way between the prefix tree's tiers: work enqueued on `stream` from here on may
 // touch the device pages they leave or land on, so it waits for the transfers (until they are
@@ -248,11 +254,8 @@ static bkv_status wait_for_table_scatter(bkv_pool* p, hipStream_t stream, bool m
 // All that was pending is written by kernels on the stream.
 static bkv_status tables_pushed(bkv_pool* p, hipStream_t stream) {
     p->alloc->pending_settled();
-    if (!p->table_sync.ev) BKV_HIP(hipEventCreateWithFlags(&p->table_sync.ev, hipEventDisableTiming));
-    BKV_HIP(hipEventRecord(p->table_sync.ev, stream));
     p->table_sync.last = stream;
-    p->table_sync.used = true;
-    return BKV_OK;
+    return record_behind(p->table_sync.ev, stream, p->table_sync.used);
 }
 
 bkv_status flush_tables(bkv_pool* p, hipStream_t stream) {
@@ -657,9 +660,12 @@ constexpr int32_t kIdsInSlot = (int32_t)(ParamRing::kSlotBytes / sizeof(int32_t)
 // One launch and no copy: of 16 sequences of 500 to 2000 cells 5, 4 layers, the host has 13 us to do, not 20, and of one 10, not 22.  The
 // kernels read the pinned memory where it is, 2 to 5 us longer than a copy of it; the copy and its gap cost as much (48 layers of 16
 // sequences, 256 cells of each: 178 us with a copy, 176 without).
+// What can fail or time out comes ahead of the first launch.  enqueued: that is out, and tables that it writes will be written, whatever
+// the status says (a device that does not answer).  Only a call of more fresh pages than the ring's slots hold, half a million, waits
+// between its launches; if that fails they are waited for, so that no kernel fills a page that is given back.
 static bkv_status compact_rows(bkv_pool* p, int32_t n, const int32_t* seqs, const int64_t* first, const int64_t* end,
                                const uint32_t* cells_dev, int64_t layer_stride, int64_t head_stride, const std::vector<int32_t>& fresh,
-                               const std::vector<int32_t>& words, size_t n_ids, hipStream_t stream) {
+                               const std::vector<int32_t>& words, size_t n_ids, hipStream_t stream, bool& enqueued) {
     CompactBatch b{};
     int64_t list = 0, pages = 0;
     int32_t at_old = 0;
@@ -678,24 +684,44 @@ static bkv_status compact_rows(bkv_pool* p, int32_t n, const int32_t* seqs, cons
         list += end[i] - first[i];
     }
     b.pages[b.n] = (int32_t)pages;
-    void* mem;
-    int slot;
+    enqueued = false;
+    (void)hipGetLastError();  // an error that others left is not one of the launches
+    void* mem[ParamRing::kSlots];
+    int slot[ParamRing::kSlots];
     if (n_ids) {
-        bkv_status st = ring_put(p, words.data(), words.size() * sizeof(int32_t), &mem, &slot);
+        bkv_status st = ring_put(p, words.data(), words.size() * sizeof(int32_t), &mem[0], &slot[0]);
         if (st != BKV_OK) return st;
-        const int32_t* const ids = static_cast<const int32_t*>(mem);
+        const int32_t* const ids = static_cast<const int32_t*>(mem[0]);
         BKV_HIP(launch_compact(p, b, ids, cells_dev, layer_stride, head_stride, 0, (int32_t)pages, ids + at_old,
                                reinterpret_cast<const TableUpdate*>(ids + n_ids), (int32_t)((words.size() - n_ids) / 2), stream));
-        return ring_done(p, slot, stream);
+        enqueued = true;
+        return ring_done(p, slot[0], stream);
     }
-    for (int32_t at = 0; at < pages; at += kIdsInSlot) {
-        const int32_t m = (int32_t)std::min<int64_t>(kIdsInSlot, pages - at);
-        bkv_status st = ring_put(p, fresh.data() + at, (size_t)m * sizeof(int32_t), &mem, &slot);
-        if (st != BKV_OK) return st;
-        BKV_HIP(launch_compact(p, b, p->table_dev, cells_dev, layer_stride, head_stride, at, m, static_cast<const int32_t*>(mem), nullptr, 0,
-                               stream));
-        st = ring_done(p, slot, stream);
-        if (st != BKV_OK) return st;
+    const auto some = [&](int32_t from, int32_t to) {
+        const auto count = [&](int32_t at) { return std::min(kIdsInSlot, to - at); };
+        bkv_status st = BKV_OK;
+        int k = 0;
+        for (int32_t at = from; at < to; at += kIdsInSlot, ++k) {
+            st = ring_put(p, fresh.data() + at, (size_t)count(at) * sizeof(int32_t), &mem[k], &slot[k]);
+            if (st != BKV_OK) return st;
+        }
+        k = 0;
+        for (int32_t at = from; at < to; at += kIdsInSlot, ++k) {
+            BKV_HIP(launch_compact(p, b, p->table_dev, cells_dev, layer_stride, head_stride, at, count(at), static_cast<const int32_t*>(mem[k]),
+                                   nullptr, 0, stream));
+            enqueued = true;
+            st = ring_done(p, slot[k], stream);
+            if (st != BKV_OK) return st;
+        }
+        return BKV_OK;
+    };
+    constexpr int32_t kOneTurn = kIdsInSlot * ParamRing::kSlots;
+    for (int32_t at = 0; at < pages; at += kOneTurn) {
+        const bkv_status st = some(at, (int32_t)std::min<int64_t>(pages, (int64_t)at + kOneTurn));
+        if (st == BKV_OK) continue;
+        if (enqueued) (void)hipDeviceSynchronize();
+        enqueued = false;  // the tables are as they were, and so is the sequence
+        return st;
     }
     return BKV_OK;
 }
@@ -749,8 +775,8 @@ bkv_status bkv_seq_compact(bkv_pool* p, int32_t n, const int32_t* seqs, const in
         }
     }
     if (e != AllocErr::Ok) return from_alloc(e, err);
-    bool pushed = false;
     if (!p->host_only && !fresh.empty()) {
+        bool pushed = false, enqueued = false;
         // (off the pages that come and go between the tiers, too)
         bkv_status st = wait_for_tier_moves(p, S(stream));
         if (st == BKV_OK) st = wait_for_table_scatter(p, S(stream), true);
@@ -767,19 +793,27 @@ bkv_status bkv_seq_compact(bkv_pool* p, int32_t n, const int32_t* seqs, const in
             pushed = words.size() <= (size_t)kIdsInSlot;
             if (st == BKV_OK && !pushed) st = flush_tables(p, S(stream));
             if (st == BKV_OK)
-                st = compact_rows(p, n, seqs, first, end, cells_dev, layer_stride, head_stride, fresh, words, pushed ? n_ids : 0, S(stream));
+                st = compact_rows(p, n, seqs, first, end, cells_dev, layer_stride, head_stride, fresh, words, pushed ? n_ids : 0, S(stream),
+                                  enqueued);
         } catch (const std::bad_alloc&) {
             st = fail(BKV_ERR_NOMEM, "seq_compact: out of host memory");
         }
-        if (st != BKV_OK) {
+        if (st != BKV_OK && !enqueued) {
             p->alloc->compact_abort(fresh);
             return st;
         }
+        // only once the kernels are enqueued does the sequence change
+        p->alloc->compact_commit(n, seqs, first, end, fresh);
+        if (pushed) {
+            const bkv_status pushed_st = tables_pushed(p, S(stream));
+            return st != BKV_OK ? st : pushed_st;
+        }
+    } else {
+        p->alloc->compact_commit(n, seqs, first, end, fresh);
     }
-    // only once the kernels are enqueued does the sequence change; entries that they do not write follow them
-    p->alloc->compact_commit(n, seqs, first, end, fresh);
-    if (pushed) return tables_pushed(p, S(stream));
-    return p->host_only ? BKV_OK : flush_tables(p, S(stream));
+    // entries that no kernel has written follow; what cannot be pushed now stays pending, and goes ahead of the next call
+    if (!p->host_only) (void)flush_tables(p, S(stream));
+    return BKV_OK;
 }
 
 // ---- prefix tree ----------------------------------------------------------------------------

@@ -159,7 +159,8 @@ bkv_status bkv_seq_truncate(bkv_pool *pool, int32_t seq, int64_t new_len);
  * a holder: forks and cached prefixes keep theirs as they were.  That takes as many free pages as the moved cells lie on
  * (cached prefixes make room as for bkv_seq_reserve; BKV_ERR_NO_PAGES, nothing changed, when that is not enough).  n_keep[i] = 0
  * only lets pages go.  BKV_ERR_STATE if a page of the sequence is swapped out, or the stream is being captured; step plans made for
- * the sequence before are void, and so is what the caller keeps of its cells (bkv_idx_pool's pooled keys).  Pages that lost their last
+ * the sequence before are void, and so is what the caller keeps of its cells (bkv_idx_pool's pooled keys).  After an error the sequences
+ * are as they were (unless the device has stopped answering behind the launch, BKV_ERR_HIP).  Pages that lost their last
  * holder are free at once: a call on another stream that writes them (whatever is written there next) has to be ordered behind this
  * one's stream, and behind work that still reads them, as for bkv_seq_free. */
 bkv_status bkv_seq_compact(bkv_pool *pool, int32_t n, const int32_t *seqs, const int64_t *first, const int32_t *n_keep,
@@ -592,8 +593,9 @@ bkv_status bkv_swap_fence(bkv_pool *pool, void *stream);
  * napping 50 us between queries (default 4000 us: a thread asleep in hipStreamSynchronize is
  * woken tens of microseconds late, which a decode loop that waits per token would pay every
  * time; 0 = never spin).  The exceptions are the device-wide synchronisations HIP offers no
- * query for: pool destruction and reset, growing the selection workspace, and the one before
- * prefix pages leave the device. */
+ * query for: pool destruction and reset, growing the selection workspace, the one before
+ * prefix pages leave the device, and the one behind an event that could not be recorded or a
+ * compaction of more than half a million pages that fails between its launches. */
 bkv_status bkv_stream_wait(void *stream, int64_t timeout_ms);
 bkv_status bkv_swap_wait_for(bkv_pool *pool, int64_t timeout_ms);
 bkv_status bkv_wait_options(int64_t timeout_ms, int64_t poll_us);
