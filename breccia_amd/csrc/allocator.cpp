@@ -75,7 +75,7 @@ void PageAllocator::set_entry(int32_t seq, int32_t col, int32_t value) {
     if (table_[off] == value) return;
     table_[off] = value;
     if (dirty_[off]) return;
-    pending_.push_back(TableUpdate{(int32_t)off, value});
+    pending_.push_back(TableUpdate{(uint32_t)off, value});
     dirty_[off] = 1;
 }
 
@@ -386,9 +386,9 @@ void PageAllocator::compact_updates(int32_t n, const int32_t* seqs, const int64_
     }
     out.reserve(out.size() + 2 * (pending_.size() + entries));
     for (const TableUpdate& u : pending_) {
-        const int32_t seq = u.offset / max_pages_per_seq_, col = u.offset - seq * max_pages_per_seq_;
+        const int32_t seq = (int32_t)(u.offset / (uint32_t)max_pages_per_seq_), col = (int32_t)(u.offset % (uint32_t)max_pages_per_seq_);
         if (col >= changed[(size_t)seq] && col < seqs_[(size_t)seq].n_pages) continue;
-        out.push_back(u.offset);
+        out.push_back((int32_t)u.offset);
         out.push_back(table_[(size_t)u.offset]);
     }
     size_t at = 0;

@@ -23,7 +23,7 @@ struct PagePair {
 // One (row, column) -> value change of the device block-table arena that has not
 // been pushed to the GPU yet.
 struct TableUpdate {
-    int32_t offset;  // row * max_pages_per_seq + column
+    uint32_t offset;  // row * max_pages_per_seq + column
     int32_t value;
 };
 

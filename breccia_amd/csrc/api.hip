@@ -421,6 +421,9 @@ bkv_status bkv_pool_create(const bkv_pool_desc* d, bkv_pool** out) {
         return fail(BKV_ERR_INVALID, sfmt("pool_create: the e4m3 layout is built for head_dim 256, not %lld", d->head_dim));
     if ((int64_t)d->n_pages * d->page_cells >= (int64_t)1 << 31)
         return fail(BKV_ERR_INVALID, "pool_create: n_pages * page_cells must stay below 2^31");
+    if ((int64_t)d->max_seqs * d->max_pages_per_seq >= (int64_t)1 << 32)
+        return fail(BKV_ERR_INVALID, sfmt("pool_create: block tables of %lld x %lld entries; their changes are named by 32 bits", d->max_seqs,
+                                          d->max_pages_per_seq));
 
     bkv_pool* p = new (std::nothrow) bkv_pool();
     if (!p) return fail(BKV_ERR_NOMEM, "pool_create: out of host memory");

@@ -83,7 +83,7 @@ typedef struct bkv_pool_desc {
     int32_t page_cells;         /* 16 */
     int32_t layout;             /* bkv_layout */
     int32_t max_seqs;           /* live sequences the block-table arena holds */
-    int32_t max_pages_per_seq;  /* block-table row length */
+    int32_t max_pages_per_seq;  /* block-table row length; max_seqs of them have fewer than 2^32 entries */
     uint32_t flags;             /* BKV_POOL_* */
 } bkv_pool_desc;
 
