@@ -23,6 +23,7 @@ PageAllocator::PageAllocator(int32_t n_pages, int32_t page_cells, int32_t max_se
       refcount_((size_t)n_pages, 0),
       external_((size_t)n_pages, 0),
       seqs_((size_t)max_seqs),
+      compacted_from_((size_t)max_seqs, max_pages_per_seq),
       table_((size_t)max_seqs * (size_t)max_pages_per_seq, -1),
       dirty_((size_t)max_seqs * (size_t)max_pages_per_seq, 0) {
     for (int32_t p = 0; p < n_pages; ++p) free_.push_back(p);
@@ -376,18 +377,17 @@ void PageAllocator::compact_columns(int32_t seq, int64_t first, int64_t end, int
 }
 
 void PageAllocator::compact_updates(int32_t n, const int32_t* seqs, const int64_t* first, const int64_t* end,
-                                    const std::vector<int32_t>& fresh, std::vector<int32_t>& out) const {
-    std::vector<int32_t> changed((size_t)max_seqs_, max_pages_per_seq_);  // from which column on
+                                    const std::vector<int32_t>& fresh, std::vector<int32_t>& out) {
     size_t entries = 0;
+    for (int32_t i = 0; i < n; ++i) entries += (size_t)seqs_[(size_t)seqs[i]].n_pages;
+    out.reserve(out.size() + 2 * (pending_.size() + entries));
     for (int32_t i = 0; i < n; ++i) {
         int32_t pages;
-        compact_columns(seqs[i], first[i], end[i], changed[(size_t)seqs[i]], pages);
-        entries += (size_t)(seqs_[(size_t)seqs[i]].n_pages - changed[(size_t)seqs[i]]);
+        compact_columns(seqs[i], first[i], end[i], compacted_from_[(size_t)seqs[i]], pages);
     }
-    out.reserve(out.size() + 2 * (pending_.size() + entries));
     for (const TableUpdate& u : pending_) {
         const int32_t seq = (int32_t)(u.offset / (uint32_t)max_pages_per_seq_), col = (int32_t)(u.offset % (uint32_t)max_pages_per_seq_);
-        if (col >= changed[(size_t)seq] && col < seqs_[(size_t)seq].n_pages) continue;
+        if (col >= compacted_from_[(size_t)seq] && col < seqs_[(size_t)seq].n_pages) continue;
         out.push_back((int32_t)u.offset);
         out.push_back(table_[(size_t)u.offset]);
     }
@@ -399,6 +399,7 @@ void PageAllocator::compact_updates(int32_t n, const int32_t* seqs, const int64_
             out.push_back(seqs[i] * max_pages_per_seq_ + c);
             out.push_back(c < pages ? fresh[at++] : -1);
         }
+        compacted_from_[(size_t)seqs[i]] = max_pages_per_seq_;
     }
 }
 

@@ -49,7 +49,7 @@ public:
     void compact_abort(const std::vector<int32_t>& fresh);
     // What would be pending after commit: offset, value, offset, value, ... behind what stands in `out`.
     void compact_updates(int32_t n, const int32_t* seqs, const int64_t* first, const int64_t* end, const std::vector<int32_t>& fresh,
-                         std::vector<int32_t>& out) const;
+                         std::vector<int32_t>& out);
     // Eviction bookkeeping: pages [lp0, lp0+n) must be complete, resident and
     // exclusively owned.  detach returns their physical ids and frees them.
     AllocErr seq_detach_pages(int32_t seq, int32_t lp0, int32_t n, std::vector<int32_t>& phys_out,
@@ -118,6 +118,7 @@ private:
     std::vector<int32_t> external_;  // part of refcount_ held by non-sequence owners
     std::deque<int32_t> free_;  // FIFO: the longest-free page is reused first
     std::vector<Seq> seqs_;
+    std::vector<int32_t> compacted_from_;  // within compact_updates: the first column that changes; max_pages_per_seq between calls
     std::vector<int32_t> table_;  // [max_seqs][max_pages_per_seq], -1 = none
     std::vector<TableUpdate> pending_;
     std::vector<uint8_t> dirty_;  // of the table's entries: among pending_
