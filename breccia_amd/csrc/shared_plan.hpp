@@ -142,7 +142,9 @@ inline bool plan_shared(const SharedPlanLimits& lim, int32_t n_groups, const int
     // Ranges of walks from .. to - 1, `least` page pairs or more each, so that they are no more than fit work-groups (one a unit if that
     // is more) and their partial results find room.  With many blocks there may be more of them once ranges have `most` pairs: one long
     // walk among short ones would have a range or two otherwise (62 entries, one with 33603 cells of its own: 480 us / 47).
-    // -> pairs of a range, or -1
+    // -> pairs of a range, or -1.  The longer the ranges, the fewer: the shortest that will do are found in steps twice as long each and
+    // then between the last two, a dozen looks at all walks at most (pair by pair up to thousands: of 200000 random batches the slowest took
+    // 1200 us of the host, now 17).
     int64_t wgs = 0, slots = 0;
     const auto cut = [&](int32_t from, int32_t to, int64_t fit, int64_t least, int64_t most, int64_t room) {
         int64_t total = 0, units = 0, longest = 1;
@@ -153,7 +155,8 @@ inline bool plan_shared(const SharedPlanLimits& lim, int32_t n_groups, const int
             longest = std::max<int64_t>(longest, pairs_of(i));
         }
         const int64_t wgs0 = wgs, slots0 = slots;
-        for (int64_t each = std::max<int64_t>({least, (total + fit - 1) / fit, least_pairs(longest)});; ++each) {
+        bool holds = false;
+        const auto does = [&](int64_t each) {
             wgs = wgs0, slots = slots0;
             for (int32_t i = from; i < to; ++i) {
                 int32_t even;
@@ -164,10 +167,25 @@ inline bool plan_shared(const SharedPlanLimits& lim, int32_t n_groups, const int
                 wgs += mine;
                 slots += mine * (plan.entries[i] * lim.group <= 16 ? 1 : plan.rows_per_wg / 16);
             }
-            const bool holds = slots <= room;
-            if (holds && wgs - wgs0 <= std::max(fit, units) + (each >= most && 4 * units > fit ? std::min(fit, units) : 0)) return each;
-            if (each >= longest) return holds ? each : (int64_t)-1;
+            holds = slots <= room;
+            return holds && wgs - wgs0 <= std::max(fit, units) + (each >= most && 4 * units > fit ? std::min(fit, units) : 0);
+        };
+        int64_t each = std::max<int64_t>({least, (total + fit - 1) / fit, least_pairs(longest)}), short_of = each - 1;
+        for (int64_t step = 1; !does(each); step *= 2) {
+            if (each >= longest) {  // one range each
+                if (!holds) return (int64_t)-1;
+                break;
+            }
+            short_of = each;
+            each = std::min(each + step, longest);
         }
+        int64_t looked_at = each;
+        while (each - short_of > 1) {
+            looked_at = short_of + (each - short_of) / 2;
+            (does(looked_at) ? each : short_of) = looked_at;
+        }
+        if (looked_at != each) (void)does(each);
+        return each;
     };
     const int64_t own_slots = (int64_t)lim.n_kv * (plan.n - plan.groups);
     const int64_t beside = plan.own_walks && (quantised || work <= 10 * (int64_t)n_cu) ? std::min<int64_t>(own_slots, n_cu / 4) : 0;
