@@ -459,7 +459,9 @@ class Pool:
         pos0, pp = _i64(pos0)
         n_tokens, pn = _i32(n_tokens)
         assert seqs.size == pos0.size == n_tokens.size
-        pair_axis = np.ascontiguousarray(pair_axis, np.uint8)
+        pair_axis = np.asarray(pair_axis)
+        # what no byte holds is an axis that there is not, not the one that its low bits name
+        pair_axis = np.ascontiguousarray(np.where((pair_axis < 0) | (pair_axis > 255), 255, pair_axis), np.uint8)
         assert pair_axis.size * 2 == n_rot
         check(lib.bkv_append_kprep_axes(self.handle, layer, seqs.size, ps, pp, pn, _ptr(k_dev), _ptr(v_dev), _ptr(gamma_dev), eps,
                                         _ptr(table_dev), n_rot, max_pos, int(pair_axis.max()) + 1 if pair_axis.size else 1,
