@@ -1,4 +1,6 @@
 """Axes of pairs that no byte holds reach the library as an axis that no call has (it refuses those), not as the one that their low bits name."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -10,7 +12,7 @@ ADDR = 0x1000  # never touched
 def handed_over(monkeypatch, pair_axis):
     """The number of axes and the axis of each pair, as the library gets them."""
     got = []
-    monkeypatch.setattr(kv.lib, "bkv_append_kprep_axes", lambda *a: got.append((a[13], [a[14][i] for i in range(4)])) or 0)
+    monkeypatch.setattr(kv.lib, "bkv_append_kprep_axes", lambda *a: got.append((a[13], list((C.c_uint8 * 4).from_address(C.addressof(a[14]))))) or 0)
     with kv.Pool(n_pages=8, max_seqs=1, host_only=True) as p:
         p.append_kprep_axes(0, [0], [0], [1], ADDR, ADDR, ADDR, 1e-6, ADDR, 8, 16, pair_axis, ADDR, 1)
     return got[0]
