@@ -21,7 +21,10 @@ struct F8Prep {
     int32_t n_rot, max_pos;
 };
 constexpr int kPrepStride = kF8Hd + 4;
-// AXES: the position of a pair is that of the token on the pair's axis.  2073 tokens of 4 kv heads: 13.7 us, 12.8 with one position a cell.
+// AXES: the position of a pair is that of the token on the pair's axis.  2073 tokens of 4 kv heads, 64 pairs: 13.1 us, 12.4 with one position
+// a cell.  Five work-groups a compute unit, all there at once: the chain of trips and barriers that each goes through.  Of the 13.1, with
+// the squares of four elements in place of 256 11.0, with one pair in place of 64 11.7, with both 9.3; rows that stay in their pages cost
+// nothing that shows (13.2 without).
 struct F8PrepAxes : F8Prep {
     KPrepAxes axes;
 };

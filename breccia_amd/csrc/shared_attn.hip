@@ -45,9 +45,10 @@ constexpr int kMergeGroups = kMergeWaves * 4;  // 16 lanes, 4 columns each, take
 // exp2(x - ref), and 0 where nothing has been attended yet (both -inf)
 __device__ __forceinline__ float weight_of(float x, float ref) { return __builtin_amdgcn_exp2f(x - (ref == -INFINITY ? 0.0f : ref)); }
 
-// A work-group per (entry, q head, quarter of the columns), as in decode_attn_merge_kernel (decode_attn.hip).  A row has up to 256
-// partial results of shared pages and a few of its own; a quarter of the waves' lanes takes every 16th.  512 rows of 35 partial results
-// 7 us, 18 MB that lie in the caches: two trips to memory (maxima and sums, rows), a launch and two barriers.
+// A work-group per (entry, q head, quarter of the columns), as in decode_attn_merge_kernel (decode_attn.hip).  A row has up to
+// kMaxSharedRanges partial results of shared pages and, of its own, up to as many from walks or what the decode kernels cut a long part
+// into; most have a few.  A quarter of a wave's lanes takes every 16th.  512 rows of 35 partial results 7 us, 18 MB that lie in the
+// caches: two trips to memory (maxima and sums, rows), a launch and two barriers.
 template <int N>
 __global__ __launch_bounds__(64 * kMergeWaves) void shared_merge_kernel(const SharedMergeArgs<N> P) {
     __shared__ __attribute__((aligned(16))) float red[kMergeWaves][kMergeCols];

@@ -59,6 +59,12 @@ inline int32_t shared_blocks(const SharedPlanLimits& lim, int32_t entries, int32
 //       64 of 4096 32.9 / 26.3, 64 of 16384 86 / 50
 //       int8: 8 of 4096 15.9 / 19, 64 of 512 18.9 / 28.6, 16 of 8192 and 1000 of their own 32 / 41 (apart); 8 of 32768 60 / 35, 64 of 4096
 //       52 / 38, 64 of 16384 161 / 72
+//       q8_0 V goes by int8's constants: 2 of 8192 15.3 / 16.3, 16 of 1024 15.7 / 23.4, 64 of 512 21.8 / 28.0, 32 of 2048 24.7 / 27.7, 16 of
+//       4096 25.0 / 27.0 (apart); 4 of 32768 44.5 / 27.2, 64 of 4096 58.5 / 40.9, 64 of 16384 180 / 66; its K need not be decoded, so a pair
+//       costs less and there are calls apart that sharing would help: 8 of 8192 25.1 / 23.4, 4 of 16384 24.7 / 21.4, 2 of 32768 28.0 / 25.7
+//   What it comes to: of 4902 drawn batches that share, 104 are more than 1 us slower than each for itself, 322 us of the 448 ms that they take
+//   apart (175 shared).  f16 49 of 3337, at worst 66 / 83; int8 5 of 606, 31 / 34; e4m3 50 of 959: dozens of own parts of a
+//   hundred cells behind 1400 shared ones, whose walks it takes to cost what f16's do, 31 / 45.  q8_0 V 33 of 2475, 86 / 99.
 //   Where the own pages are read apart the call is two launches behind, 13 us, and on e4m3 pools, whose pages are small, 20: 32 of 8192
 //   and 4000 of their own, f16 89 / 60, int8 71 / 67, e4m3 47 / 52 (with 13).
 // - Blocks of 64 rows, and of 128 (quantised pools: always) where the walks are long: such a block takes 1.57 us a pair, two of 64 1.9.
@@ -66,7 +72,8 @@ inline int32_t shared_blocks(const SharedPlanLimits& lim, int32_t entries, int32
 //   122 / 102, 90 / 80.
 // - Own pages by walks, in the same launch, or by the decode kernels: 5 us a call for the start of another kernel; but a walk of 16 rows
 //   uses a quarter of a work-group.  By walks / apart: f16, 32 of 8192 and 4000 of their own 61 / 70, 64 of 4096 and 100 of their own
-//   28 / 35, 8 of 8192 with 8 others of 30000 beside them 114 / 98; e4m3 56 / 52, 30 / 35, 110 / 63; int8 90 / 65, 38 / 44, 134 / 74.  A wave
+//   28 / 35, 8 of 8192 with 8 others of 30000 beside them 114 / 98; e4m3 56 / 52, 30 / 35, 110 / 63; int8 90 / 65, 38 / 44, 134 / 74; q8_0 V
+//   87 / 73, 41 / 42, 16 of 16384 and 4000 of their own 62 / 58.  A wave
 //   of 512 registers leaves no room for another work-group: blocks of 128 rows leave the own pages apart, on quantised pools unless all is
 //   short.
 // - As many ranges as compute units: a second work-group a unit brings little (the products bound it: 64 rows a pair 0.94 us alone, 0.88

@@ -139,7 +139,7 @@ bkv_status bkv_seq_free(bkv_pool *pool, int32_t seq);
  * and partially filled, it is replaced by a fresh page and (old, new) is reported in
  * cow_pairs -- the caller must bkv_page_copy those pairs before appending.  A shared
  * page that no other sequence holds any more (refcount back to 1) is written in place.
- * On BKV_ERR_NO_PAGES nothing is changed. */
+ * On BKV_ERR_NO_PAGES no sequence has changed (cached prefixes may have been evicted for it). */
 bkv_status bkv_seq_reserve(bkv_pool *pool, int32_t seq, int64_t new_len, bkv_page_pair *cow_pairs,
                            int32_t cow_capacity, int32_t *n_cow);
 /* Set the sequence's length without touching pages (speculative rollback:
@@ -157,7 +157,8 @@ bkv_status bkv_seq_truncate(bkv_pool *pool, int32_t seq, int64_t new_len);
  * back, would leave there (rows in front of first[i] in the same page among them).
  * The rows are moved into fresh pages, from the page of cell first[i] on; what stood there, and every page behind the new end, loses
  * a holder: forks and cached prefixes keep theirs as they were.  That takes as many free pages as the moved cells lie on
- * (cached prefixes make room as for bkv_seq_reserve; BKV_ERR_NO_PAGES, nothing changed, when that is not enough).  n_keep[i] = 0
+ * (cached prefixes make room as for bkv_seq_reserve; BKV_ERR_NO_PAGES when that is not enough: no sequence has changed then, but the
+ * prefixes that had to go are evicted or on a lower tier).  n_keep[i] = 0
  * only lets pages go.  BKV_ERR_STATE if a page of the sequence is swapped out, or the stream is being captured; step plans made for
  * the sequence before are void, and so is what the caller keeps of its cells (bkv_idx_pool's pooled keys).  After an error the sequences
  * are as they were (unless the device has stopped answering behind the launch, BKV_ERR_HIP).  Pages that lost their last
@@ -497,9 +498,11 @@ bkv_status bkv_decode_attn_select(bkv_pool *pool, int32_t layer, int32_t n, cons
  * whole page that they share.  A group of one entry, or with no cells, is an ordinary one.
  * Same result as bkv_decode_attn but for the order of sums (and a sum that is no number makes NaN, on every layout); same shapes, checks
  * and limits.  Entries of one sequence with different pos may stand in one group, which reads that sequence's pages once.
- * A call whose sharing would not save what it costs -- few entries, few pages -- is bkv_decode_attn itself, bit for bit
+ * A call whose sharing is not expected to save what it costs -- few entries, few pages -- is bkv_decode_attn itself, bit for bit
  * (bkv_shared_plan says which); so is one on a stream that is being captured, or of a pool without memory for the partial results, which
- * lie in a workspace of bkv_prefill_attn, with its ordering across streams.  All layouts.
+ * lie in a workspace of bkv_prefill_attn, with its ordering across streams.  All layouts.  What is expected is an estimate from lengths
+ * and shapes: a call near the border may be slower shared than it would be apart (of 7377 random batches that share 137 are, by more than
+ * 1 us; dozens of short own parts on an e4m3 pool took 45 us, not 31).  group_cells of 0 keep a group apart.
  * bkv_shared_plan: what a call on a device of n_cu compute units would do, worked out on the host without pool or device.
  * pages_out[n_groups]: pages of group g that are read once (0: none); *total_out: work-groups of the launch that does it, 0 where the
  * call is bkv_decode_attn. */
