@@ -100,8 +100,8 @@ static int64_t default_timeout_ms() { return g_wait_timeout_ms.load(std::memory_
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- parameter ring ---------------------------------------------------------------
-// `bytes` of host data in a slot's pinned memory, where a kernel may read it in place: every time over the bus, past the caches.  A list that is
-// read once costs less so than its copy; page ids that every layer and kv head looks up are even (compact_rows).
+// `bytes` of host data in a slot's pinned memory, where a kernel may read it in place.  A list that is read once costs less so than with a
+// copy to the device first; page ids that every layer and kv head of a compaction looks up, in no order, as much (compact_rows).
 static bkv_status ring_put(bkv_pool* p, const void* host_src, size_t bytes, void** host_out, int* slot_out) {
     ParamRing& r = p->ring;
     if (bytes > ParamRing::kSlotBytes)
